@@ -6,6 +6,8 @@
   * ``jax_llama_amd/_C_hybrid*.so`` — the hybrid-mixer kernels (``csrc/hybrid/*.hip``: row-gathered / expert-grouped
     linears, biased soft-capped attention, the gated delta rule) + their bindings; small, self-contained, and the
     only native code the hybrid model family needs (``--only hybrid`` builds it alone in about a minute);
+  * ``jax_llama_amd/_C_serving*.so`` — the serving kernels (``csrc/serving/*.hip``: attention over shared prefixes,
+    penalties and masks on logits, copies of cache rows) + their bindings (``--only serving``);
   * ``jax_llama_amd/_bpe*.so`` — the C++ byte-pair-merge core of the Llama-3 tokenizer.
 
 The xGMI custom all-reduce (``csrc/kernels/allreduce.hip``) is part of ``_C``.
@@ -13,7 +15,7 @@ The xGMI custom all-reduce (``csrc/kernels/allreduce.hip``) is part of ``_C``.
 No hipify, no CUDA, no JIT cache: objects go to ``build/`` (incremental, mtime based) and the
 final ``.so`` files land next to the Python package so they travel with the repo snapshot.
 
-Usage: ``python build.py [-j N] [--force] [--only C|hybrid|bpe] [--debug-bounds]``
+Usage: ``python build.py [-j N] [--force] [--only C|hybrid|serving|bpe] [--debug-bounds]``
 
 ``--debug-bounds`` additionally builds ``jax_llama_amd/_C_dbg*.so`` (objects in ``build/C_dbg``) with
 ``-DJLA_DEBUG_BOUNDS``: every clamped / skipped out-of-range index that comes from device state (token ids,
@@ -76,8 +78,8 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-f
              "-Wno-unused-result", "-D__HIP_PLATFORM_AMD__"]
 # A source's own flags. delta_chunk: with a wave per SIMD the compiler puts the products' sums into the matrix unit's own registers, and
 # the 64 of a chunk that are added up pass through a move each (2048 tokens of 16 heads of 128 x 128, delta rule 210 -> 195 us, scalar gates 121 -> 111).
-# rows_mid, linear_mid: they are copied out of those registers and back at the loop's edge otherwise.
-FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("delta_chunk", "rows_mid", "linear_mid")}
+# rows_mid, linear_mid, prefix_attn: they are copied out of those registers and back at the loop's edge otherwise.
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("delta_chunk", "rows_mid", "linear_mid", "prefix_attn")}
 
 
 def _scratch_users(remarks: str):
@@ -188,24 +190,33 @@ def _link(out: Path, objs, force: bool):
               "-lamdhip64", f"-Wl,-rpath,{tlib}"])
 
 
-def build_hybrid(jobs: int, force: bool) -> Path:
-    """``_C_hybrid``: csrc/hybrid/*.hip + csrc/hybrid/bindings.cpp (its own module, so a hybrid model runs without
-    compiling the LLaMA kernels)."""
-    hdir = CSRC / "hybrid"
-    headers = sorted(hdir.glob("*.h")) + [CSRC / "kernels" / h for h in ("common.h", "gemm4w.h", "row_tiles.h", "gemm_f32x3.h", "mid_tile.h")]
+def _build_module(name: str, hdir: Path, shared, jobs: int, force: bool) -> Path:
+    """Module ``name``: the sources and ``bindings.cpp`` of ``hdir``, which use the headers ``shared`` of csrc/kernels."""
+    headers = sorted(hdir.glob("*.h")) + [CSRC / "kernels" / h for h in shared]
     srcs = sorted(hdir.glob("*.hip"))
-    odir = BUILD / "C_hybrid"
+    odir = BUILD / name[1:]
     objs = [odir / (s.stem + ".o") for s in srcs]
     bobj = odir / "bindings.o"
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         futs = [ex.submit(_compile_hip, s, o, headers, force) for s, o in zip(srcs, objs)]
-        bind = ex.submit(_compile_bindings, hdir / "bindings.cpp", bobj, headers, "_C_hybrid", force)
+        bind = ex.submit(_compile_bindings, hdir / "bindings.cpp", bobj, headers, name, force)
         rebuilt = [f.result() for f in futs]
         bind.result()
     _check_asm(zip(srcs, objs, rebuilt), odir, jobs)
-    out = PKG / f"_C_hybrid{EXT_SUFFIX}"
+    out = PKG / f"{name}{EXT_SUFFIX}"
     _link(out, [*objs, bobj], force)
     return out
+
+
+def build_hybrid(jobs: int, force: bool) -> Path:
+    """``_C_hybrid``: csrc/hybrid/*.hip + csrc/hybrid/bindings.cpp (its own module, so a hybrid model runs without
+    compiling the LLaMA kernels)."""
+    return _build_module("_C_hybrid", CSRC / "hybrid", ("common.h", "gemm4w.h", "row_tiles.h", "gemm_f32x3.h", "mid_tile.h"), jobs, force)
+
+
+def build_serving(jobs: int, force: bool) -> Path:
+    """``_C_serving``: csrc/serving/*.hip + csrc/serving/bindings.cpp."""
+    return _build_module("_C_serving", CSRC / "serving", ("common.h",), jobs, force)
 
 
 def build_bpe(force: bool) -> Path:
@@ -223,6 +234,8 @@ def build_all(jobs: int = 8, force: bool = False, only=None, debug_bounds: bool 
         outs.append(build_bpe(force))
     if only in (None, "hybrid"):
         outs.append(build_hybrid(jobs, force))
+    if only in (None, "serving"):
+        outs.append(build_serving(jobs, force))
     if only in (None, "C"):
         outs.append(build_C(jobs, force))
         if debug_bounds:
@@ -234,7 +247,7 @@ if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("-j", type=int, default=min(8, os.cpu_count() or 4))
     ap.add_argument("--force", action="store_true")
-    ap.add_argument("--only", choices=["C", "hybrid", "bpe"])
+    ap.add_argument("--only", choices=["C", "hybrid", "serving", "bpe"])
     ap.add_argument("--debug-bounds", action="store_true", help="also build the bounds-checked _C_dbg extension")
     a = ap.parse_args()
     for o in build_all(a.j, a.force, a.only, a.debug_bounds):

@@ -13,7 +13,23 @@ is run to create it (unlike the reference's ``module.init`` trick).
 """
 from __future__ import annotations
 
+from typing import Optional, Sequence
+
 import torch
+
+from ..ops import cache_rows
+
+
+def _copy_rows(cache, src, dst, tokens, to) -> None:
+    target = cache if to is None else to
+    if type(target) is not type(cache):
+        raise ValueError(f"rows of a {type(cache).__name__} go to a {type(cache).__name__}, not to a {type(target).__name__}")
+    tokens = cache.index if tokens is None else int(tokens)
+    if not 0 <= tokens <= min(cache.max_length, target.max_length):
+        raise ValueError(f"{tokens} tokens of rows of {cache.max_length} and {target.max_length}")
+    src, dst = [int(r) for r in src], [int(r) for r in dst]
+    cache_rows.check_pairs(src, dst, cache.batch_size, target.batch_size)
+    cache_rows.copy_rows(cache.row_layout(), target.row_layout(), src, dst, tokens)
 
 
 class KVCache:
@@ -27,10 +43,24 @@ class KVCache:
         self.max_length = max_length
         self.index = 0  # host mirror of the number of filled slots
         self.index_t = torch.zeros(1, dtype=torch.int32, device=device)
+        self._row_layout = None
 
     @property
     def device(self):
         return self.k.device
+
+    def row_layout(self) -> cache_rows.RowLayout:
+        at = (self.k.data_ptr(), self.v.data_ptr())
+        if self._row_layout is None or self._row_layout[0] != at:
+            self._row_layout = at, cache_rows.RowLayout([(x, True) for i in range(self.k.shape[0]) for x in self.layer(i)])
+        return self._row_layout[1]
+
+    def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None, to: Optional["KVCache"] = None) -> None:
+        """Row ``dst[i]`` becomes row ``src[i]`` (-1: zeros) in every layer, its first ``tokens`` tokens (default: as many as the cache
+        holds by its host counter): forks, reordering, moving live rows to the front. Every source is read as it was before the call; a row is
+        written once at most. ``to``: the rows written are those of another cache with the same layers (whose slot counter stays as it is).
+        One launch; up to some 400 rows also while a stream is captured, once the caches have copied rows before."""
+        _copy_rows(self, src, dst, tokens, to)
 
     def layer(self, i: int):
         return self.k[i], self.v[i]
@@ -132,6 +162,7 @@ class HybridCache:
             for part in self.parts(sp):
                 self._alloc(i, part, batch_size, max_length, dtype, device)
         self._device = device
+        self._row_layout = None
         self.index = 0
         self.index_t = torch.zeros(1, dtype=torch.int32, device=device)
         # counters of the one-launch decode steps (ops.hybrid.attn_step, delta_step), which leave them at zero: part of the cache because
@@ -192,6 +223,16 @@ class HybridCache:
     @property
     def device(self):
         return self._device
+
+    def row_layout(self) -> cache_rows.RowLayout:
+        if self._row_layout is None:
+            held = [(t, True) for t in {id(t): t for d in (self._k, self._v) for t in d.values()}.values()]
+            self._row_layout = cache_rows.RowLayout(held + [(t, False) for d in (self._state, self._conv) for t in d.values()])
+        return self._row_layout
+
+    def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None, to: Optional["HybridCache"] = None) -> None:
+        """``KVCache.copy_rows``, with the rows' whole recurrent state."""
+        _copy_rows(self, src, dst, tokens, to)
 
     def layer(self, i: int):
         """Keys and values layer ``i`` attends over (its own, or the layer's it shares them with)."""

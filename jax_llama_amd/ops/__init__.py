@@ -19,6 +19,7 @@ from . import autotune
 from . import reference as ref
 from ._ext import available as ext_available  # noqa: F401
 from ._ext import ext
+from .serving import pack_allowed, prefix_attention, process_logits  # noqa: F401
 from .slots import slot_tensor as _slot_tensor
 
 BF16 = torch.bfloat16
