@@ -25,6 +25,7 @@ from .models.fokisun import FokisunForCausalLM
 from .models.zopupel import ZopupelForCausalLM
 from .models.zavevik import ZavevikForCausalLM
 from .runtime.engine import GenerationConfig
+from .runtime.logit_rules import TokenGrammar
 from .runtime.stepper import SequenceStepper
 from .tokenizer import ChatFormat, LLaMA2Tokenizer, LLaMA3Tokenizer
 from .utils.checkpoint import convert_llama_weights
@@ -34,7 +35,7 @@ __version__ = "0.1.0"
 __all__ = [
     "LLaMAConfig", "ModelArgs", "config_from_params", "get_preset", "swiglu_hidden_size",
     "LLaMA", "LLaMAForCausalLM", "LLaMAModel", "FlaxLLaMAForCausalLM", "FlaxLLaMAModel",
-    "CausalLMOutput", "KVCache", "GenerationConfig",
+    "CausalLMOutput", "KVCache", "GenerationConfig", "TokenGrammar",
     "Mesh", "P", "PartitionSpec", "get_llama_param_partition_spec", "with_named_sharding_constraint",
     "with_sharding_constraint", "LLaMA2Tokenizer", "LLaMA3Tokenizer", "ChatFormat", "convert_llama_weights",
     "ZavevikConfig", "ZavevikForCausalLM", "ZasevikConfig", "ZasevikForCausalLM", "BesulixConfig", "BesulixForCausalLM",

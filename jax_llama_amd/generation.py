@@ -30,7 +30,8 @@ class LLaMA:
         self.mesh = mesh
 
     def generate(self, tokens, attention_mask, max_gen_len: int, temperature: float = 0.8,
-                 top_p: float = 0.95, seed: int = 0) -> torch.Tensor:
+                 top_p: float = 0.95, seed: int = 0, **settings) -> torch.Tensor:
+        """``settings``: further fields of ``GenerationConfig`` (``num_return_sequences``, ``repetition_penalty``, ``grammar``, ...)."""
         tokens = torch.as_tensor(tokens, dtype=torch.int32) if not torch.is_tensor(tokens) else tokens
         attention_mask = (torch.as_tensor(attention_mask, dtype=torch.int32)
                           if not torch.is_tensor(attention_mask) else attention_mask)
@@ -45,6 +46,7 @@ class LLaMA:
             temperature=temperature,
             top_p=top_p,
             seed=seed,
+            **settings,
         )
         out = self.model.generate(tokens, attention_mask=attention_mask, generation_config=gc)
         # the reference's output constraint P("dp", None) keeps the batch split across dp replicas;
@@ -52,21 +54,23 @@ class LLaMA:
         return gather_dp(out.sequences, self.mesh)
 
     def generate_from_str(self, prompts: List[str], max_gen_len: int, temperature: float = 0.8,
-                          top_p: float = 0.95, seed: int = 0) -> List[str]:
+                          top_p: float = 0.95, seed: int = 0, **settings) -> List[str]:
+        """``settings`` as in ``generate``; of several sequences per prompt a prompt's stand next to each other."""
         tok = self.tokenizer
+        each = int(settings.get("num_return_sequences", 1))
         prompt_tokens = [tok.encode(x, bos=True, eos=False) for x in prompts]
         max_prompt = max(len(t) for t in prompt_tokens)
         tokens = torch.full((len(prompts), max_prompt), tok.eos_id, dtype=torch.int32)
         for i, t in enumerate(prompt_tokens):
             tokens[i, max_prompt - len(t):] = torch.tensor(t, dtype=torch.int32)  # left pad
         attention_mask = (tokens != tok.eos_id).to(torch.int32)
-        out_tokens = self.generate(tokens, attention_mask, max_gen_len, temperature, top_p, seed)
+        out_tokens = self.generate(tokens, attention_mask, max_gen_len, temperature, top_p, seed, **settings)
         # rows of this dp replica only when the outputs could not be gathered (no process group)
-        row0 = 0 if out_tokens.shape[0] == len(prompts) else self.mesh.dp_rank * out_tokens.shape[0]
+        row0 = 0 if out_tokens.shape[0] == len(prompts) * each else self.mesh.dp_rank * out_tokens.shape[0]
         decoded = []
         for i, t in enumerate(out_tokens.tolist()):
             t = t[t.index(tok.bos_id):]
-            t = t[: len(prompt_tokens[row0 + i]) + max_gen_len]
+            t = t[: len(prompt_tokens[(row0 + i) // each]) + max_gen_len]
             try:
                 t = t[: t.index(tok.eos_id)]
             except ValueError:

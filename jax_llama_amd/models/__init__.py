@@ -1,4 +1,4 @@
-from .kv_cache import KVCache
+from .kv_cache import KVCache, SharedPrefixCache
 from .llama import BaseModelOutput, CausalLMOutput, LLaMAForCausalLM, LLaMAModel, mask_to_kv_start
 from .modules import LLaMAAttention, LLaMABlock, LLaMABlockCollection, LLaMAMLP
 from .weights import PackedLinear
@@ -11,7 +11,7 @@ FlaxLLaMAMLP = LLaMAMLP
 FlaxLLaMABlock = LLaMABlock
 FlaxLLaMABlockCollection = LLaMABlockCollection
 
-__all__ = ["KVCache", "LLaMAForCausalLM", "LLaMAModel", "FlaxLLaMAForCausalLM", "FlaxLLaMAModel",
+__all__ = ["KVCache", "SharedPrefixCache", "LLaMAForCausalLM", "LLaMAModel", "FlaxLLaMAForCausalLM", "FlaxLLaMAModel",
            "LLaMAAttention", "LLaMAMLP", "LLaMABlock", "LLaMABlockCollection", "FlaxLLaMAAttention",
            "FlaxLLaMAMLP", "FlaxLLaMABlock", "FlaxLLaMABlockCollection",
            "CausalLMOutput", "BaseModelOutput", "PackedLinear", "mask_to_kv_start"]

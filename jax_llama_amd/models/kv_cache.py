@@ -43,6 +43,7 @@ class KVCache:
         self.max_length = max_length
         self.index = 0  # host mirror of the number of filled slots
         self.index_t = torch.zeros(1, dtype=torch.int32, device=device)
+        self.start: Optional[torch.Tensor] = None  # int32 [B]: a left-padded prefix's first real slot of each row (``encode_prefix``)
         self._row_layout = None
 
     @property
@@ -123,6 +124,78 @@ class KVCacheRows:
 
     def layer(self, i: int):
         return self.parent.k[i, self.b0:self.b1], self.parent.v[i, self.b0:self.b1]
+
+    def rows(self, b0: int, b1: int) -> "KVCacheRows":
+        return KVCacheRows(self.parent, self.b0 + b0, self.b0 + b1)
+
+
+class SharedPrefixCache:
+    """A batch's own cache behind prefixes that its rows share: row ``b`` of ``B`` continues row ``b // (B / G)`` of ``prefix`` (a KVCache of
+    ``G`` rows holding the prefixes' keys and values, read once for all of a prefix's rows: ``ops.prefix_attention``). Slots, ``index`` and
+    ``layer(i)`` are those of ``own``; positions go on where the prefix ends. ``start`` / ``mask``: the prefixes' first keys (int32
+    ``[G]``) and the keys that count (uint8 ``[G, capacity]``). Anything that writes here writes to ``own`` alone."""
+
+    def __init__(self, prefix: KVCache, own, start: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
+        if own.batch_size % prefix.batch_size:
+            raise ValueError(f"{own.batch_size} rows are not a multiple of {prefix.batch_size} prefixes")
+        if prefix.device != own.device:
+            raise ValueError(f"the prefixes lie on {prefix.device}, the rows on {own.device}")
+        self.prefix, self.own, self.start, self.mask = prefix, own, start if start is not None else prefix.start, mask
+        self.prefix_len = torch.full((prefix.batch_size,), prefix.index, dtype=torch.int32, device=prefix.device)
+        self.batch_size, self.max_length = own.batch_size, own.max_length
+
+    @property
+    def device(self):
+        return self.own.device
+
+    @property
+    def index(self):
+        return self.own.index
+
+    @index.setter
+    def index(self, n):
+        self.own.index = n
+
+    @property
+    def index_t(self):
+        return self.own.index_t
+
+    def layer(self, i: int):
+        return self.own.layer(i)
+
+    def prefix_layer(self, i: int):
+        return self.prefix.layer(i)
+
+    def advance(self, n: int) -> None:
+        self.own.advance(n)
+
+    def reset(self) -> None:
+        self.own.reset()
+
+    def clear(self) -> None:
+        self.own.clear()
+
+    def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None) -> None:
+        """``KVCache.copy_rows`` of the own rows; a row only goes to rows of its own prefix."""
+        n = self.batch_size // self.prefix.batch_size
+        if any(a >= 0 and a // n != b // n for a, b in zip(src, dst)):
+            raise ValueError("a row would continue another prefix")
+        self.own.copy_rows(src, dst, tokens)
+
+    def rows(self, b0: int, b1: int) -> "SharedPrefixCache":
+        """Rows ``[b0, b1)``: whole prefixes' rows, or some of one prefix's."""
+        n = self.batch_size // self.prefix.batch_size
+        g0, g1 = b0 // n, -(-b1 // n)
+        if g1 - g0 > 1 and (b0 % n or b1 % n):
+            raise ValueError(f"rows {b0} .. {b1 - 1} hold some of one prefix's rows and others")
+        part = SharedPrefixCache.__new__(SharedPrefixCache)
+        part.prefix, part.own = self.prefix.rows(g0, g1), self.own.rows(b0, b1)
+        part.start, part.mask = (t[g0:g1] if t is not None else None for t in (self.start, self.mask))
+        part.prefix_len, part.batch_size, part.max_length = self.prefix_len[g0:g1], b1 - b0, self.max_length
+        return part
+
+    def nbytes(self) -> int:
+        return self.own.nbytes()
 
 
 TICKET_INTS = 64 * 32  # tickets of a cache row that has some: 64, each on a line of its own (csrc: AS_TICKET)
@@ -330,6 +403,9 @@ class HybridCacheRows:
     def layer(self, i: int):
         k, v = self.parent.layer(i)
         return k[self.b0:self.b1], v[self.b0:self.b1]
+
+    def rows(self, b0: int, b1: int) -> "HybridCacheRows":
+        return HybridCacheRows(self.parent, self.b0 + b0, self.b0 + b1)
 
     def owns_kv(self, i: int) -> bool:
         return self.parent.owns_kv(i)

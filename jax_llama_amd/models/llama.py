@@ -33,7 +33,7 @@ from ..ops import reference as ref
 from ..ops.slots import step_slot
 from ..parallel.comm import NO_COMM, TPComm
 from ..parallel.partition import shard_tree
-from .kv_cache import KVCache
+from .kv_cache import KVCache, SharedPrefixCache
 from .modules import LLaMABlockCollection
 from .weights import PackedLinear
 
@@ -137,6 +137,7 @@ class LLaMAForCausalLM:
 
     base_model_prefix = "transformer"
     config_class = LLaMAConfig
+    shares_prefixes = True  # forward_tokens takes a SharedPrefixCache
 
     def __init__(self, config: LLaMAConfig, input_shape: Tuple[int, ...] = (1, 1), seed: int = 0, dtype=None,
                  _do_init: bool = True, precision=None, param_dtype=None, device="cpu",
@@ -327,6 +328,35 @@ class LLaMAForCausalLM:
         return KVCache(self.config.num_hidden_layers, batch_size, self.n_kv_heads, max_length,
                        self.head_dim, self.device)
 
+    def encode_prefix(self, input_ids, attention_mask=None) -> KVCache:
+        """The keys and values of prefixes ``[G, P]`` (a system prompt, a document) for ``generate(prefix=...)`` and ``share_prefix``.
+        ``attention_mask``: of left-padded prefixes."""
+        ids = _t(input_ids).to(self.device, torch.int32)
+        g, p = ids.shape
+        cache = self.init_cache(g, p)
+        if attention_mask is None:
+            pos = torch.arange(p, dtype=torch.int32, device=self.device).expand(g, p).contiguous()
+            start = torch.zeros(g, dtype=torch.int32, device=self.device)
+        else:
+            mask = _t(attention_mask).to("cpu", torch.int32)
+            if tuple(mask.shape) != (g, p):
+                raise ValueError(f"attention_mask of shape {tuple(mask.shape)} for prefixes {(g, p)}")
+            start, holes = mask_to_kv_start(mask, self.device)
+            if holes is not None:
+                raise ValueError("a prefix may be padded on the left only")
+            cache.start = start
+            pos = (mask.cumsum(-1) - 1).to(torch.int32).to(self.device)
+        self.forward_tokens(ids, pos, cache, 0, start, logits_mode="none")
+        cache.advance(p)
+        return cache
+
+    def share_prefix(self, prefix: KVCache, batch_size: int, max_length: int) -> SharedPrefixCache:
+        """A cache of ``batch_size`` rows (``past_key_values``) of ``max_length`` own tokens each behind the prefixes in ``prefix``; row ``b``
+        continues prefix ``b // (batch_size / G)``. Positions go on at the prefix's number of real tokens."""
+        if prefix.index + max_length > self.rope_length:
+            raise ValueError(f"{prefix.index} + {max_length} tokens exceed the RoPE table ({self.rope_length})")
+        return SharedPrefixCache(prefix, self.init_cache(batch_size, max_length))
+
     # ------------------------------------------------------------------ core forward
     def _row_parallel(self, x: torch.Tensor, w: PackedLinear, h: torch.Tensor, hb: torch.Tensor,
                       x_packed: Optional[torch.Tensor] = None, mirror_packed: Optional[torch.Tensor] = None) -> None:
@@ -481,8 +511,9 @@ class LLaMAForCausalLM:
 
     def generate(self, input_ids, attention_mask=None, generation_config=None, params=None,
                  prng_key=None, **kwargs):
-        """HF ``generate`` equivalent (greedy / sampling with temperature, top-k, top-p),
-        executed by the hipGraph decode engine (``runtime/engine.py``)."""
+        """HF ``generate`` equivalent (greedy / sampling with temperature, top-k, top-p; several samples per prompt; penalties,
+        biases and grammars, ``GenerationConfig``), executed by the hipGraph decode engine (``runtime/engine.py``). ``prefix=``: a cache
+        with prefixes that the prompts continue (``encode_prefix``)."""
         from ..runtime.engine import generate as _generate
         if params is not None and id(params) != self._params_id:
             self.load_params(params)

@@ -39,6 +39,8 @@ class LLaMAAttention:
                  output_attentions: bool = False, pk: Optional["PackedActs"] = None) -> Optional[torch.Tensor]:
         m, lw = self.model, self.weights
         kc, vc = cache.layer(self.layer_idx)
+        if getattr(cache, "prefix", None) is not None:
+            return self._behind_prefix(h, hb, positions, cache, slot0, kv_start, key_mask, seq_len, output_attentions, pk)
         splits = og = 0
         o_state = None
         if not output_attentions:
@@ -81,6 +83,23 @@ class LLaMAAttention:
         if pk is not None and pk.hb is not None:
             pk.hb_ok = True
         return weights
+
+
+    def _behind_prefix(self, h, hb, positions, cache, slot0, kv_start, key_mask, seq_len, output_attentions, pk) -> None:
+        """Rows that continue shared prefixes (``models.kv_cache.SharedPrefixCache``)."""
+        if output_attentions or key_mask is not None:
+            raise NotImplementedError("behind shared prefixes: rows without holes, no attention maps")
+        m, lw = self.model, self.weights
+        kc, vc = cache.layer(self.layer_idx)
+        q = ops.linear_qkv_rope(hb, lw.qkv, m.eps, m.rope, positions, kc, vc, slot0, seq_len, m.n_heads, m.n_kv_heads, m.head_dim,
+                                x_packed=pk.hb_in() if pk else None)
+        att_p = pk.att if pk is not None else None
+        a = ops.prefix_attention(q.reshape(-1, seq_len, m.n_heads, m.head_dim), *cache.prefix_layer(self.layer_idx), kc, vc, slot0,
+                                 prefix_len=cache.prefix_len, prefix_start=cache.start, prefix_mask=cache.mask, kv_start=kv_start,
+                                 out_packed=att_p)
+        m._row_parallel(a, lw.o, h, hb, x_packed=att_p, mirror_packed=pk.hb if pk else None)
+        if pk is not None and pk.hb is not None:
+            pk.hb_ok = True
 
 
 class LLaMAMLP:

@@ -41,6 +41,14 @@ def ext():
     return _EXT
 
 
+def ext_available() -> bool:
+    try:
+        ext()
+        return True
+    except RuntimeError:
+        return False
+
+
 def _need(ok: bool, msg: str) -> None:
     if not ok:
         raise ValueError(msg)

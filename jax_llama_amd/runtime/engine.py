@@ -27,11 +27,13 @@ import dataclasses
 import os
 from collections import OrderedDict
 from dataclasses import dataclass
-from typing import Optional
+from typing import Dict, List, Optional, Union
 
 import torch
 
 from .. import ops
+from ..models.kv_cache import KVCache, SharedPrefixCache
+from .logit_rules import LogitRules, TokenGrammar
 from ..ops import reference as ref
 
 _NEG_INF = float("-inf")
@@ -39,7 +41,10 @@ _NEG_INF = float("-inf")
 
 @dataclass
 class GenerationConfig:
-    """Subset of HF ``GenerationConfig`` used by the reference (``generation.py:32-40``)."""
+    """Subset of HF ``GenerationConfig`` used by the reference (``generation.py:32-40``), and how the logits are changed before a token is
+    chosen (``ops.process_logits``, in this order): ``repetition_penalty`` on the tokens of prompt and continuation,
+    ``frequency_penalty`` / ``presence_penalty`` on those of the continuation, ``logit_bias`` (token -> number, or fp32 ``[V]``) and
+    ``suppress_tokens``, ``grammar``. ``num_return_sequences``: sampled continuations of each prompt, next to each other in the result."""
 
     max_length: Optional[int] = None
     max_new_tokens: Optional[int] = None
@@ -51,6 +56,13 @@ class GenerationConfig:
     pad_token_id: Optional[int] = None
     eos_token_id: Optional[int] = None
     seed: int = 0
+    num_return_sequences: int = 1
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Union[Dict[int, float], torch.Tensor, None] = None
+    suppress_tokens: Optional[List[int]] = None
+    grammar: Optional[TokenGrammar] = None
 
 
 # prompt tokens per prefill forward (DecodeEngine._prefill_rows): larger batches run their prefill in row chunks
@@ -127,11 +139,17 @@ def _sample(model, logits_local: torch.Tensor, gc: GenerationConfig, gen: Option
 
 # --------------------------------------------------------------------------------------
 class DecodeEngine:
-    """Owns the KV cache and the device-resident decode state for one (B, max_length)."""
+    """Owns the KV cache and the device-resident decode state for one (B, max_length).
+
+    ``samples``: continuations of each of ``batch_size`` prompts. Where the model attends over shared prefixes
+    (``shares_prefixes``: LLaMA) the prompts are such prefixes, held and read once (``prompt_len`` fixes their length); else the prompts'
+    cache rows are copied. ``prefix``: a cache with prefixes that the prompts continue (``LLaMAForCausalLM.encode_prefix``)."""
 
     def __init__(self, model, batch_size: int, max_length: int, use_graph: Optional[bool] = None,
-                 check_every: int = 16):
+                 check_every: int = 16, samples: int = 1, prompt_len: int = 0, prefix: Optional[KVCache] = None):
         self.model = model
+        self.prompts, self.samples = batch_size, samples
+        batch_size *= samples
         self.b = batch_size
         self.max_length = max_length
         dev = model.device
@@ -140,7 +158,21 @@ class DecodeEngine:
             use_graph = dev.type == "cuda" and os.environ.get("JLA_NO_GRAPH", "0") != "1"
         self.use_graph = use_graph
         self.check_every = check_every
-        self.cache = model.init_cache(batch_size, max_length)
+        self.prefix = prefix
+        self.prompt_cache: Optional[KVCache] = None
+        if prefix is not None:
+            self.cache = model.share_prefix(prefix, batch_size, max_length)
+        elif samples > 1 and getattr(model, "shares_prefixes", False):
+            self.prompt_cache = model.init_cache(self.prompts, prompt_len)
+            self.prompt_start = torch.zeros(self.prompts, dtype=torch.int32, device=dev)
+            self.prompt_mask = torch.zeros(self.prompts, prompt_len, dtype=torch.uint8, device=dev)
+            if max_length > model.rope_length:
+                raise ValueError(f"max_length {max_length} exceeds the RoPE table ({model.rope_length}); raise config.max_sequence_length")
+            self.cache = SharedPrefixCache(self.prompt_cache, model.init_cache(batch_size, max_length - prompt_len), self.prompt_start)
+            self.cache.prefix_len.fill_(prompt_len)
+        else:
+            self.cache = model.init_cache(batch_size, max_length)
+        self.rules = LogitRules(model, batch_size, max_length)
         i32 = dict(dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(batch_size, 1, **i32)
         self.positions = torch.zeros(batch_size, 1, **i32)
@@ -157,9 +189,11 @@ class DecodeEngine:
 
     # ---------------------------------------------------------------------------------
     def _next_token(self, logits_local):
-        if self.gc.do_sample:
-            return _sample(self.model, logits_local, self.gc, self._gen, self.cur_len)
-        return _greedy(self.model, logits_local)
+        if self.rules.any:
+            logits_local = self.rules.apply(logits_local, self.sequences, self.cur_len)
+        nxt = _sample(self.model, logits_local, self.gc, self._gen, self.cur_len) if self.gc.do_sample else _greedy(self.model, logits_local)
+        self.rules.chosen(nxt)
+        return nxt
 
     def _update(self, nxt: torch.Tensor):
         """Device-side HF loop-body bookkeeping (pad for finished rows, eos tracking,
@@ -181,7 +215,7 @@ class DecodeEngine:
         self.cur_len.add_(1)
 
     def _logits_mode(self) -> str:
-        return "argmax" if _fused_greedy() and not self.gc.do_sample else "last"
+        return "argmax" if _fused_greedy() and not self.gc.do_sample and not self.rules.any else "last"
 
     def _decode_step(self):
         mode = self._logits_mode()
@@ -198,42 +232,76 @@ class DecodeEngine:
 
     # ---------------------------------------------------------------------------------
     def prefill(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor]):
-        model, dev = self.model, self.device
+        model, dev, n = self.model, self.device, self.samples
         ids = input_ids.to(dev, torch.int32)
         b, s = ids.shape
-        assert b == self.b and s < self.max_length
+        assert b == self.prompts and s < self.max_length
         if attention_mask is None:  # every key of every row: positions on the device, nothing to look through on the host
             pos_dev = torch.arange(s, dtype=torch.int32, device=dev).expand(b, s).contiguous()
-            self.kv_start.zero_()
-            self.key_mask = None
+            start, key_mask = torch.zeros(b, dtype=torch.int32, device=dev), None
         else:
             mask = attention_mask.to("cpu", torch.int32)
             pos_dev = (mask.cumsum(-1) - 1).to(torch.int32).to(dev)
             ext_mask = torch.ones(b, self.max_length, dtype=torch.int32)
             ext_mask[:, :s] = mask
             from ..models.llama import mask_to_kv_start
-            kv_start, key_mask = mask_to_kv_start(ext_mask, dev)
-            self.kv_start.copy_(kv_start)
-            self.key_mask = key_mask
+            start, key_mask = mask_to_kv_start(ext_mask, dev)
+        if self.prefix is not None:
+            self._behind_prefix()
+            if key_mask is not None:
+                raise ValueError("prompts behind a prefix may be padded on the left only")
+            before = self.cache.prefix_len - (self.cache.start if self.cache.start is not None else 0)
+            pos_dev = pos_dev + before.repeat_interleave(b // self.prefix.batch_size)[:, None]
+
+        def each(t):  # a prompt's to all of its rows
+            return t if n == 1 else t.repeat_interleave(n, 0)
+
+        self.rules.begin(self.gc, s, each(start), each(key_mask) if key_mask is not None else None)
         self.cache.reset()
         self.sequences.fill_(self.gc.pad_token_id)
-        self.sequences[:, :s] = ids
+        self.sequences[:, :s] = each(ids)
         self.finished.zero_()
-        logits = self._prefill_rows(ids, pos_dev)
-        self.cache.advance(s)
+        held = s  # own slots the prompts take
+        if self.prompt_cache is not None:
+            self.prompt_cache.reset()
+            self.prompt_start.copy_(start)
+            self.kv_start.zero_()
+            self.key_mask = None
+            self.cache.mask = None if key_mask is None else self.prompt_mask.copy_(key_mask[:, :s])
+            logits = self._prefill_rows(ids, pos_dev, self.prompt_cache, start, key_mask)
+            self.prompt_cache.advance(s)
+            held = 0
+        else:
+            self.kv_start.copy_(each(start))
+            self.key_mask = key_mask
+            if n == 1:
+                logits = self._prefill_rows(ids, pos_dev, self.cache, self.kv_start, key_mask)
+            else:
+                own = self.cache.own if self.prefix is not None else self.cache
+                rows = own.rows(0, b)
+                logits = self._prefill_rows(ids, pos_dev, SharedPrefixCache(self.prefix, rows) if self.prefix is not None else rows, start, None)
+                own.copy_rows([i // n for i in range(self.b)], range(self.b), tokens=s)
+        self.cache.advance(held)
         # state for the loop body: cur_len = S (also the sampler's Philox step), token/pos of the
         # last prompt position
         self.cur_len.fill_(s)
-        nxt = self._next_token(logits)
-        self.positions.copy_(pos_dev[:, -1:])
-        # _update writes sequences[:, S], advances pos (+1), slot (+1 -> S+1 ... ) and cur_len.
-        # The prefill already advanced the slot by S; undo the update's +1 on the slot.
+        nxt = self._next_token(tuple(each(x) for x in logits) if isinstance(logits, tuple) else each(logits))
+        self.positions.copy_(each(pos_dev[:, -1:]))
+        # _update writes sequences[:, S], advances pos (+1), slot (+1 -> held+1 ... ) and cur_len.
+        # The prefill already advanced the slot; undo the update's +1 on the slot.
         self.cache.index_t.sub_(1)
         self._update(nxt)
-        self.cache.index = s  # host mirror (decode steps track the slot on the device)
+        self.cache.index = held  # host mirror (decode steps track the slot on the device)
         return s + 1
 
-    def _prefill_rows(self, ids: torch.Tensor, pos_dev: torch.Tensor):
+    def _behind_prefix(self) -> None:
+        """The prefix as it is now (its owner may have extended it since the last call)."""
+        if self.prefix.index + self.max_length > self.model.rope_length:
+            raise ValueError(f"{self.prefix.index} + {self.max_length} tokens exceed the RoPE table ({self.model.rope_length})")
+        self.cache.prefix_len.fill_(self.prefix.index)
+        self.cache.start = self.prefix.start
+
+    def _prefill_rows(self, ids: torch.Tensor, pos_dev: torch.Tensor, cache, kv_start: torch.Tensor, key_mask: Optional[torch.Tensor]):
         """The prompt forward, in row chunks of at most PREFILL_TOKENS tokens: every kernel then sees at most the
         token count the GEMMs already saturate the chip with (M = 262144: 2048 rows x 128), whatever the batch, and no
         activation index of a larger batch can pass 2^31 elements. One chunk up to that size (the common case)."""
@@ -241,16 +309,18 @@ class DecodeEngine:
         rows = max(1, PREFILL_TOKENS // max(1, s))
         mode = self._logits_mode()
         if b <= rows:
-            logits, *_ = self.model.forward_tokens(ids, pos_dev, self.cache, 0, self.kv_start, self.key_mask,
-                                                   logits_mode=mode)
+            logits, *_ = self.model.forward_tokens(ids, pos_dev, cache, 0, kv_start, key_mask, logits_mode=mode)
             return logits
+        group = b // cache.prefix.batch_size if isinstance(cache, SharedPrefixCache) else 1  # (chunks of whole groups, or within one)
+        if rows >= group:
+            rows, group = rows - rows % group, b
         parts = []
-        for b0 in range(0, b, rows):
-            b1 = min(b, b0 + rows)
-            km = self.key_mask[b0:b1] if self.key_mask is not None else None
-            lg, *_ = self.model.forward_tokens(ids[b0:b1], pos_dev[b0:b1], self.cache.rows(b0, b1), 0,
-                                               self.kv_start[b0:b1], km, logits_mode=mode)
-            parts.append(lg)
+        for g0 in range(0, b, group):
+            for b0 in range(g0, g0 + group, rows):
+                b1 = min(g0 + group, b0 + rows)
+                km = key_mask[b0:b1] if key_mask is not None else None
+                lg, *_ = self.model.forward_tokens(ids[b0:b1], pos_dev[b0:b1], cache.rows(b0, b1), 0, kv_start[b0:b1], km, logits_mode=mode)
+                parts.append(lg)
         if isinstance(parts[0], tuple):  # greedy: (idx, val) per chunk
             return tuple(torch.cat([p[i] for p in parts]) for i in range(len(parts[0])))
         return torch.cat(parts)
@@ -263,7 +333,16 @@ class DecodeEngine:
     def _graph_state(self):
         # the graph records buffer addresses: the scratch workspaces (ops.workspace) and the sampling mode
         return (self.gc.do_sample, self.key_mask is not None, ops.workspace.generation, _fused_greedy(),
-                ops.ARGMAX_FUSED_MIN_M, ops.SKINNY_ARGMAX, ops.QKV_ATTN, self.model.comm.reduce_dtype)
+                ops.ARGMAX_FUSED_MIN_M, ops.SKINNY_ARGMAX, ops.QKV_ATTN, self.model.comm.reduce_dtype, self.rules.key(), self._prefix_state())
+
+    def _prefix_state(self):
+        if not isinstance(self.cache, SharedPrefixCache):
+            return None
+        c = self.cache
+        return (c.prefix.k.data_ptr(), c.prefix.v.data_ptr(), *(t.data_ptr() if t is not None else 0 for t in (c.start, c.mask)))
+
+    def nbytes(self) -> int:
+        return self.cache.nbytes() + (self.prompt_cache.nbytes() if self.prompt_cache is not None else 0)
 
     def _ensure_graph(self):
         if self._graph is not None and self._graph_key == self._graph_state():
@@ -317,6 +396,8 @@ class DecodeEngine:
             # engine's cache beyond where the next prompt writes; the kernels mask keys past the valid length by
             # probability 0, and 0 x NaN is NaN: zero the cache so the next call starts as from a fresh engine
             self.cache.clear()
+            if self.prompt_cache is not None:
+                self.prompt_cache.clear()
             raise
         finally:
             if rng_saved is not None:
@@ -358,31 +439,36 @@ def _engine_budget(model) -> int:
     return 8 << 30
 
 
-def get_engine(model, batch_size: int, max_length: int) -> DecodeEngine:
-    """Per-(model, B, max_length) engines (each owns a KV cache and a captured decode graph), kept in
-    LRU order and bounded by the bytes of their KV caches."""
-    key = (id(model), batch_size, max_length)
+def get_engine(model, batch_size: int, max_length: int, samples: int = 1, prompt_len: int = 0, prefix: Optional[KVCache] = None) -> DecodeEngine:
+    """Per-(model, B, max_length) engines (each owns a KV cache and a captured decode graph; of several samples per prompt, and behind a
+    prefix, engines of their own), kept in LRU order and bounded by the bytes of their KV caches."""
+    shared = samples > 1 and prefix is None and getattr(model, "shares_prefixes", False)
+    key = (id(model), batch_size, max_length, samples, prompt_len if shared else 0, id(prefix) if prefix is not None else 0)
     eng = _ENGINES.get(key)
     if eng is not None:
         _ENGINES.move_to_end(key)
         return eng
+    rows = batch_size * samples
     if hasattr(model, "cache_nbytes"):  # layer-list models: per-layer geometry, recurrent state
-        need = model.cache_nbytes(batch_size, max_length)
+        need = model.cache_nbytes(rows, max_length)
     else:
-        need = model.config.num_hidden_layers * 2 * batch_size * model.n_kv_heads * max_length * model.head_dim * 2
+        tokens = batch_size * prompt_len + rows * (max_length - prompt_len) if shared else rows * max_length
+        need = model.config.num_hidden_layers * 2 * tokens * model.n_kv_heads * model.head_dim * 2
     budget = _engine_budget(model)
-    held = sum(e.cache.nbytes() for e in _ENGINES.values())
+    held = sum(e.nbytes() for e in _ENGINES.values())
     while _ENGINES and held + need > budget:
         _, old = _ENGINES.popitem(last=False)
-        held -= old.cache.nbytes()
+        held -= old.nbytes()
         del old
-    eng = DecodeEngine(model, batch_size, max_length)
+    eng = DecodeEngine(model, batch_size, max_length, samples=samples, prompt_len=prompt_len, prefix=prefix)
     _ENGINES[key] = eng
     return eng
 
 
 def generate(model, input_ids, attention_mask=None, generation_config: Optional[GenerationConfig] = None,
-             prng_key=None, **kwargs) -> GenerateOutput:
+             prng_key=None, prefix: Optional[KVCache] = None, **kwargs) -> GenerateOutput:
+    """``prefix``: the prompts continue the prefixes of this cache (``LLaMAForCausalLM.encode_prefix``), prompt ``b`` of ``B`` prefix
+    ``b // (B / G)``; the result and the penalties' history hold the prompts' own tokens."""
     # never mutate the caller's config (HF semantics: generate works on a copy)
     gc = dataclasses.replace(generation_config) if generation_config is not None else GenerationConfig()
     for k, v in kwargs.items():
@@ -390,8 +476,16 @@ def generate(model, input_ids, attention_mask=None, generation_config: Optional[
             setattr(gc, k, v)
     if gc.num_beams != 1:
         raise NotImplementedError("beam search is not used by the reference (num_beams=1)")
+    n = int(gc.num_return_sequences)
+    if n < 1 or (n > 1 and not gc.do_sample):
+        raise ValueError(f"num_return_sequences = {n}: one, or several sampled ones (greedy ones would be equal)")
     ids = input_ids if torch.is_tensor(input_ids) else torch.as_tensor(input_ids)
     b, s = ids.shape
+    if prefix is not None:
+        if not getattr(model, "shares_prefixes", False):
+            raise NotImplementedError(f"{type(model).__name__} does not attend over shared prefixes")
+        if b % prefix.batch_size:
+            raise ValueError(f"{b} prompts are not a multiple of {prefix.batch_size} prefixes")
     if gc.max_length is None:
         gc.max_length = s + (gc.max_new_tokens if gc.max_new_tokens is not None else 20)
     if gc.pad_token_id is None:
@@ -403,8 +497,8 @@ def generate(model, input_ids, attention_mask=None, generation_config: Optional[
     if prng_key is not None:
         gc.seed = int(prng_key) if not torch.is_tensor(prng_key) else int(prng_key.reshape(-1)[0])
     if s >= gc.max_length:
-        return GenerateOutput(sequences=ids.to(model.device, torch.int32)[:, : gc.max_length])
-    eng = get_engine(model, b, gc.max_length)
+        return GenerateOutput(sequences=ids.to(model.device, torch.int32)[:, : gc.max_length].repeat_interleave(n, 0))
+    eng = get_engine(model, b, gc.max_length, n, s, prefix) if n > 1 or prefix is not None else get_engine(model, b, gc.max_length)
     seq = eng.run(ids, attention_mask if attention_mask is None or torch.is_tensor(attention_mask)
                   else torch.as_tensor(attention_mask), gc)
     return GenerateOutput(sequences=seq.clone())

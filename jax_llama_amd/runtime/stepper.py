@@ -4,7 +4,8 @@ The counterpart of the generation engine for replaying a trace (or scoring text)
 (keys / values of the attention layers, the recurrent layers' state) from its first portion until it ends; a portion
 runs only its own tokens on top of what the earlier portions left, through the model's step function
 (``forward_tokens``) -- the same one the engine's prefill and decode steps call. Rows are pooled: an ended request's row
-goes back to the pool and is reset when the next request takes it.
+goes back to the pool and is reset when the next request takes it. A request can be forked: what it holds is copied to
+the new request's row.
 """
 from __future__ import annotations
 
@@ -43,6 +44,17 @@ class SequenceStepper:
         if cache is not None:
             self._free.append(cache)
 
+    def fork(self, rid: str, new: str) -> None:
+        """Request ``new`` goes on where ``rid`` stands: its row becomes a copy (one launch)."""
+        if rid not in self._live:
+            raise ValueError(f"request {rid!r} is not live")
+        if new in self._live:
+            raise ValueError(f"request {new!r} is live already")
+        held = self._live[rid]
+        cache = self._row(new)
+        held.copy_rows([0], [0], to=cache)
+        cache.advance(held.index)
+
     # ---------------------------------------------------------------- steps
     def feed(self, rid: str, tokens: Sequence[int], want: Sequence[int] = ()) -> Optional[torch.Tensor]:
         """Run the next ``tokens`` of request ``rid``; returns fp32 logits ``[len(want), vocab]`` at the places ``want``
@@ -68,9 +80,11 @@ class SequenceStepper:
         cache.advance(n)
         return logits
 
-    def step(self, entries: Sequence[dict], end: Sequence[str] = ()) -> Optional[torch.Tensor]:
-        """One trace step: ``entries`` of ``{"id", "tokens", "want"}`` run in order, then the requests in ``end`` give
+    def step(self, entries: Sequence[dict], end: Sequence[str] = (), fork: Sequence[Sequence[str]] = ()) -> Optional[torch.Tensor]:
+        """One trace step: the pairs ``(request, new request)`` of ``fork`` are forked, ``entries`` of ``{"id", "tokens", "want"}`` run in order, then the requests in ``end`` give
         their rows back. Returns the wanted logits of all entries stacked (None if none)."""
+        for rid, new in fork:
+            self.fork(rid, new)
         outs = []
         for e in entries:
             lg = self.feed(e["id"], e["tokens"], e.get("want", ()))

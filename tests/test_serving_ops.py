@@ -132,7 +132,7 @@ def walk(rows, steps, chains, in_place):
 
 @pytest.mark.parametrize("seed", range(60))
 def test_row_plans(seed):
-    if not hasattr(serving, "ext") or not _has_ext():
+    if not serving.ext_available():
         pytest.skip("the extension is not built")
     rng = random.Random(seed)
     n = rng.choice([1, 2, 3, 5, 9, 40])
@@ -157,14 +157,6 @@ def test_row_plans(seed):
                 touched.append(wrote[-1] | {a for a, _ in part if a >= 0})
             for i, w in enumerate(wrote):
                 assert all(not w & t for j, t in enumerate(touched) if j != i)
-
-
-def _has_ext():
-    try:
-        serving.ext()
-        return True
-    except RuntimeError:
-        return False
 
 
 def cache_tensors(cache):
