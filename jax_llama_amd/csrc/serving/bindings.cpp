@@ -64,6 +64,7 @@ void prefix_attn(Tensor q, Tensor kp, Tensor vp, Tensor ko, Tensor vo, Tensor sl
   TORCH_CHECK(a.B > 0 && a.S > 0 && a.H > 0 && a.G > 0 && a.Hkv > 0 && a.P > 0 && a.T > 0 && a.B % a.G == 0 && a.H % a.Hkv == 0, JLA_SV,
               "prefix_attn: rows must be a multiple of the prefixes, heads of the kv heads, and none may be empty");
   TORCH_CHECK((int64_t)a.B * a.S * (a.H / a.Hkv) < (1LL << 31) && q.size(0) * q.size(1) * q.size(2) < (1LL << 33), JLA_SV, "prefix_attn: too many queries");
+  a.rep = a.H / a.Hkv, a.n = a.B / a.G;
   aligned(q, 16, "q");
   a.q = reinterpret_cast<const uint16_t*>(q.data_ptr());
   a.kp = keys(kp, q, a.G, a.Hkv, a.P, "prefix keys", &a.kp_g, &a.kp_h);

@@ -9,6 +9,8 @@
 // Columns. The queries of one kv head that read the same keys are the columns of S^T = K Q^T: for a prefix n S rep of them (n rows of
 // its group, rep query heads per kv head, column c = token (c / rep), head (c % rep)), for a row's own keys S rep. So a prefix is
 // read once per 128 columns instead of once per row.
+#include <type_traits>
+
 #include "../kernels/common.h"
 #include "serving.h"
 
@@ -65,22 +67,13 @@ JLA_DEV KeyRange own_keys(const PrefixAttn& a, int b, int kvh, int s_last) {
   return r;
 }
 
-// One part of a query head: the sums (4 of its dims from d on per call), or where there is one part the result
-JLA_DEV void put_sums(const PrefixAttn& a, int part, size_t qh, int d, const float* o) {
-  *reinterpret_cast<f32x4*>(a.part + ((size_t)part * a.B * a.S * a.H + qh) * PA_DH + d) = f32x4{o[0], o[1], o[2], o[3]};
-}
-JLA_DEV void put_stats(const PrefixAttn& a, int parts, int part, size_t qh, float m, float l) {
+// A part's share of the workspace: [parts][queries][128] sums, then [parts][queries][2] (maximum, sum of weights)
+JLA_DEV float* part_sums(const PrefixAttn& a, int part, size_t qh) { return a.part + ((size_t)part * a.B * a.S * a.H + qh) * PA_DH; }
+JLA_DEV float* part_stats(const PrefixAttn& a, int parts, int part, size_t qh) {
   const size_t n = (size_t)a.B * a.S * a.H;
-  *reinterpret_cast<float2*>(a.part + n * PA_DH * parts + (part * n + qh) * 2) = make_float2(m, l);
+  return a.part + n * PA_DH * parts + (part * n + qh) * 2;
 }
-JLA_DEV void put_result(const PrefixAttn& a, size_t qh, int d, const float* o, float inv) {
-  const u32x2 v = {pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
-  *reinterpret_cast<u32x2*>(a.out + qh * PA_DH + d) = v;
-  if (a.out_pack) {
-    const int K = a.H * PA_DH;
-    *reinterpret_cast<u32x2*>(a.out_pack + pack_off((int)(qh / a.H), (int)(qh % a.H) * PA_DH + d, K)) = v;
-  }
-}
+JLA_DEV u32x2 result4(const float* o, float inv) { return u32x2{pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)}; }
 
 // ---- 128 columns of a workgroup of four waves, 32 a wave (a lane's column is lane & 31). Tiles of 64 keys go to LDS by LDS-DMA, two
 // slots each for keys and values; S^T = K Q^T leaves a column's scores in its two lanes, which are the operand of O^T += V^T P^T as
@@ -88,14 +81,14 @@ JLA_DEV void put_result(const PrefixAttn& a, size_t qh, int d, const float* o, f
 JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int kvh, size_t tok0, int ncols, int ct, const KeyRange& pre,
                          const KeyRange& own, char* lds) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hi = lane >> 5, rep = a.H / a.Hkv;
-  const int c0 = ct * PA_COLS + 32 * w, c = min(c0 + (lane & 31), ncols - 1);
+  const int hi = lane >> 5, col = lane & 31, rep = a.rep;
+  const int c0 = (4 * ct + w) * 32;
   const bool active = c0 < ncols;  // (the wave's; the others help to stage)
-  const size_t qh = (tok0 + c / rep) * a.H + kvh * rep + c % rep;
   const float scale = 1.4426950408889634f / 11.313708498984761f;
-  // its slot; that of the wave's first column
-  const int slot = a.slot[0], at = slot + c / rep, at_first = slot + min(c0, ncols - 1) / rep;
-
+  // a column's slot; those of the wave's first and last columns
+  const int slot = a.slot[0], at_first = slot + min(c0, ncols - 1) / rep, at_last = slot + min(c0 + 31, ncols - 1) / rep;
+  const int c = min(c0 + col, ncols - 1), at = slot + c / rep;
+  const size_t qh = (tok0 + c / rep) * a.H + kvh * rep + c % rep;
   u32x4 qf[8];
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(a.q + qh * PA_DH + 16 * ks + 8 * hi);
@@ -104,127 +97,218 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = -INFINITY, m_use = 0.f, l_run = 0.f, sum = 0.f;
+  u32x4 pf = {0u, 0u, 0u, 0u};
 
   const int n_pre = pre.tiles(PA_KT), n_all = n_pre + own.tiles(PA_KT);
   const int from = (int)((long long)n_all * part / p.ns), to = (int)((long long)n_all * (part + 1) / p.ns);
-  auto stage = [&](int i) {
-    const bool is_own = i >= n_pre;
-    const KeyRange& r = is_own ? own : pre;
-    const int t0 = r.first(PA_KT) + (is_own ? i - n_pre : i) * PA_KT;
-    char* const kd = lds + (i & 1) * PA_TILE;
-    char* const vd = lds + (2 + (i & 1)) * PA_TILE;
+  const int gq = (lane & 15) >> 2, gp = lane & 3, G = lane >> 4;
+  struct Tile {
+    const bf16_t *k, *v;
+    const uint8_t* mask;
+    int t0, lo, hi, limit;
+    bool own;
+  };
+  auto tile_of = [&](int i) {
+    return i < n_pre ? Tile{pre.k, pre.v, pre.mask, pre.first(PA_KT) + i * PA_KT, pre.lo, pre.hi, pre.limit, false}
+                     : Tile{own.k, own.v, nullptr, own.first(PA_KT) + (i - n_pre) * PA_KT, own.lo, own.hi, own.limit, true};
+  };
+  // a bit for each of a tile's keys that the range and the mask leave (all lanes)
+  auto kept_of = [&](const Tile& t) -> uint64_t {
+    if (t.t0 >= t.lo && t.t0 + PA_KT <= t.hi && !t.mask) return ~0ull;
+    const int key = t.t0 + lane;
+    return __ballot(key >= t.lo && key < t.hi && (!t.mask || t.mask[min(key, t.limit - 1)]));
+  };
+  // else nothing of a tile is this wave's, nor of those after it
+  auto mine = [&](const Tile& t) { return active && (!t.own || t.t0 <= at_last); };
+  auto slot_k = [&](int par) { return lds + par * PA_TILE; };
+  auto slot_v = [&](int par) { return lds + (2 + par) * PA_TILE; };
+  // 1-KiB blocks of 4 rows, lane L fills row L / 16, place L % 16 of its block (by asm: for the builtin the compiler waits before the
+  // next read of LDS)
+  auto stage = [&](const bf16_t* src, const Tile& t, char* to_lds) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // 1-KiB blocks of 4 rows; lane L fills row L / 16, place L % 16 of its block
+    for (int j = 0; j < 4; ++j) {
       const int bi = w + 4 * j, row = 4 * bi + (lane >> 4);
       const int ch = (lane & 15) ^ (((row & 3) << 2) | ((row >> 2) & 3));
-      const int off = 256 * min(row, r.limit - 1 - t0) + 16 * ch;
-      glds16_asm(r.k + (size_t)t0 * PA_DH, off, kd + 1024 * bi);
-      glds16_asm(r.v + (size_t)t0 * PA_DH, off, vd + 1024 * bi);
+      glds16_asm(src + (size_t)t.t0 * PA_DH, 256 * min(row, t.limit - 1 - t.t0) + 16 * ch, to_lds + 1024 * bi);
     }
   };
-  const int col = lane & 31, gq = (lane & 15) >> 2, gp = lane & 3, G = lane >> 4;
-  if (from < to) stage(from);
-  wait_vmcnt<0>();
-  __syncthreads();
-  for (int i = from; i < to; ++i) {
-    if (i + 1 < to) stage(i + 1);
-    const bool is_own = i >= n_pre;
-    const KeyRange& r = is_own ? own : pre;
-    const int t0 = r.first(PA_KT) + (is_own ? i - n_pre : i) * PA_KT;
-    const char* const kt = lds + (i & 1) * PA_TILE;
-    char* const vt = lds + (2 + (i & 1)) * PA_TILE;
-    const bool edge = t0 < r.lo || t0 + PA_KT > r.hi || r.mask;  // (the workgroup's)
-    if (edge) {  // values of keys that nobody attends may be anything: 0 x NaN would not be 0
+  auto stage_k = [&](int i, int par) { const Tile t = tile_of(i); stage(t.k, t, slot_k(par)); };
+  auto stage_v = [&](int i, int par) { const Tile t = tile_of(i); stage(t.v, t, slot_v(par)); };
+
+  // Tile i: K(i + 1) and V(i) are there, K(i + 2) and V(i + 1) on their way to the slots that tile i - 1 is done with. The scores of
+  // tile i + 1 stand among the PV products of tile i, the exponentials of a key step among the products of the one before: the matrix
+  // unit (1024 cycles a tile and wave) and the vector unit (about 900) work side by side.
+  f32x16 sa[2], sb[2];
+  const int k_off = pa_off(col, hi), v_off = pa_off(4 * (G >> 1) + gq, 2 * (G & 1) + (gp >> 1)) + 8 * (gp & 1);
+  auto score = [&](f32x16 (&s)[2], const char* kt, int f) {
+    const u32x4 k = *reinterpret_cast<const u32x4*>(kt + (k_off ^ (32 * (f >> 1))) + 8192 * (f & 1));
+    s[f & 1] = mfma32(k, qf[f >> 1], s[f & 1]);
+  };
+  auto clear = [&](f32x16 (&s)[2]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = (tid >> 4) + 16 * j, key = t0 + row;
-        if (key < r.lo || key >= r.hi || (r.mask && !r.mask[key]))
-          *reinterpret_cast<u32x4*>(vt + 256 * row + 16 * (tid & 15)) = u32x4{0u, 0u, 0u, 0u};
-      }
-      __syncthreads();
+    for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
+  };
+  auto largest = [&](const f32x16 (&s)[2]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, s[kb][e]);
+    return m;
+  };
+  // weights of key step ks, in bf16 for the matrix cores (half a step, 2^-8, at most; their sum is of the unrounded ones)
+  auto weights = [&](const f32x16 (&s)[2], int ks) {
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      e[j] = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][8 * (ks & 1) + j], scale, -m_use));
+      sum += e[j];
     }
-    if (active) {
-      f32x16 s[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          s[kb] = mfma32(*reinterpret_cast<const u32x4*>(kt + pa_off(32 * kb + col, 2 * ks + hi)), qf[ks], s[kb]);
-      }
-      // element e of block kb is key t0 + 32 kb + (e & 3) + 8 (e >> 2) + 4 hi
-      if (edge || (is_own && t0 + PA_KT - 1 > at_first)) {
-        const int upto = is_own ? min(at, r.hi - 1) : r.hi - 1;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = t0 + 32 * kb + (e & 3) + 8 * (e >> 2) + 4 * hi;
-            bool ok = key >= r.lo && key <= upto;
-            if (r.mask) ok = ok && r.mask[min(key, r.limit - 1)];
-            s[kb][e] = ok ? s[kb][e] : -INFINITY;
-          }
-      }
-      float most = -INFINITY;
+    return pack8(e);
+  };
+  // what a tile needs before its PV: masks, the running maximum (it moves, and the sums with it, only where it grew by more than 8:
+  // 2^(x - m) stays below 256), the weights of its first key step. raw: the largest score before masks
+  auto enter = [&](const Tile& t, uint64_t kept, f32x16 (&s)[2], float raw) {
+    if (kept != ~0ull || (t.own && t.t0 + PA_KT - 1 > at_first)) {
+      uint64_t ok = kept;  // element e of block kb is key t0 + 4 hi + 32 kb + (e & 3) + 8 (e >> 2)
+      const int n = at - t.t0 + 1;
+      if (t.own && n < PA_KT) ok = n > 0 ? ok & ~(~0ull << n) : 0ull;
+      ok >>= 4 * hi;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) most = fmaxf(most, s[kb][e]);
-      most = lane_max32(most) * scale;
-      // the maximum moves, and the sums with it, only where it grew by more than 8: 2^(x - m) stays below 256
-      if (__ballot(most > m_run + 8.f)) {
-        const float m_new = fmaxf(m_run, most);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
-        l_run *= alpha;
-        m_run = m_new;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-      }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        float e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][8 * (ks & 1) + j], scale, -m_use));
-          l_run += e[j];
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t all = __builtin_amdgcn_sbfe((uint32_t)(ok >> (32 * kb)), (e & 3) + 8 * (e >> 2), 1);
+          s[kb][e] = __uint_as_float((__float_as_uint(s[kb][e]) & all) | (0xff800000u & ~all));
         }
-        const u32x4 pf = pack8(e);  // (bf16 weights for the matrix cores: 2^-9 of each, their sum is of the unrounded ones)
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          const int row = 16 * ks + 4 * (G >> 1) + gq, ch = 4 * dt + 2 * (G & 1) + (gp >> 1);
-          const u32x2 lo4 = ld_tr(vt, pa_off(row, ch) + 8 * (gp & 1)), hi4 = ld_tr(vt, pa_off(row + 8, ch) + 8 * (gp & 1));
-          o[dt] = mfma32(u32x4{lo4[0], lo4[1], hi4[0], hi4[1]}, pf, o[dt]);
-        }
-      }
+      raw = largest(s);
     }
+    const float most = lane_max32(raw) * scale;
+    if (__ballot(most > m_run + 8.f)) {
+      const float m_new = fmaxf(m_run, most);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+      m_run = m_new;
+      m_use = m_new == -INFINITY ? 0.f : m_new;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    sum = 0.f;
+    pf = weights(s, 0);
+  };
+  auto pv = [&](const char* vt, int ks, int dt) {
+    const u32x2 lo4 = ld_tr(vt, (v_off ^ (64 * dt)) + 4096 * ks), hi4 = ld_tr(vt, (v_off ^ (64 * dt) ^ 32) + 2048 + 4096 * ks);
+    o[dt] = mfma32(u32x4{lo4[0], lo4[1], hi4[0], hi4[1]}, pf, o[dt]);
+  };
+  uint64_t kept = ~0ull;  // tile i's
+  auto step = [&](int i, auto parity, f32x16 (&s)[2], f32x16 (&next)[2]) {
+    constexpr int par = decltype(parity)::value;
+    const Tile t = tile_of(i), tn = tile_of(min(i + 1, to - 1));
+    const uint64_t kept_next = kept_of(tn);
+    if (i + 2 < to) stage_k(i + 2, par);
+    if (i + 1 < to) stage_v(i + 1, par ^ 1);
+    if (kept != ~0ull) {  // values of keys that nobody attends may be anything: 0 x NaN would not be 0
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = (tid >> 4) + 16 * j;
+        if (!(kept >> row & 1)) *reinterpret_cast<u32x4*>(slot_v(par) + 256 * row + 16 * (tid & 15)) = u32x4{0u, 0u, 0u, 0u};
+      }
+      __syncthreads();
+    }
+    if (mine(t)) {
+      clear(next);
+#pragma unroll
+      for (int ks = 0; ks < 3; ++ks) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 6 * ks; f < (ks < 2 ? 6 * ks + 6 : 16); ++f) score(next, slot_k(par ^ 1), f);
+        const u32x4 after = weights(s, ks + 1);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) pv(slot_v(par), ks, dt);
+        pf = after;
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int j = 0; j < (ks < 2 ? 10 : 8); ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      l_run += sum;  // (this half's keys; the halves meet at the end)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) pv(slot_v(par), 3, dt);
+      const float raw = largest(next);
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + 1 < to && mine(tn)) enter(tn, kept_next, next, raw);
+    }
+    kept = kept_next;
     wait_vmcnt<0>();
     __syncthreads();
+  };
+  if (from < to) {
+    stage_k(from, 0);
+    stage_v(from, 0);
+    if (from + 1 < to) stage_k(from + 1, 1);
+    wait_vmcnt<0>();
+    __syncthreads();
+    const Tile t = tile_of(from);
+    if (mine(t)) {
+      clear(sa);
+#pragma unroll
+      for (int f = 0; f < 16; ++f) score(sa, slot_k(0), f);
+    }
+    if (from + 2 < to) __syncthreads();  // K(from + 2) goes where K(from) was
+    kept = kept_of(t);
+    if (mine(t)) enter(t, kept, sa, largest(sa));
+    for (int i = from; i < to; i += 2) {
+      step(i, std::integral_constant<int, 0>{}, sa, sb);
+      if (i + 1 < to) step(i + 1, std::integral_constant<int, 1>{}, sb, sa);
+    }
   }
-  l_run = lane_sum32(l_run);
-  if (c0 + col >= ncols) return;
+  const float l = lane_sum32(l_run);
   const int parts = p.parts();
-  const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
+  if (c0 + col >= ncols) return;
+  if (parts > 1) {
+    float* const dst = part_sums(a, part, qh) + 4 * hi;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+    if (hi == 0) *reinterpret_cast<float2*>(part_stats(a, parts, part, qh)) = make_float2(m_run, l);
+    return;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  bf16_t* const dst = a.out + qh * PA_DH + 4 * hi;
+  const int row = (int)(qh / a.H), first = (int)(qh % a.H) * PA_DH + 4 * hi;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float v[4] = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-      if (parts > 1) put_sums(a, part, qh, 32 * dt + 8 * g + 4 * hi, v);
-      else put_result(a, qh, 32 * dt + 8 * g + 4 * hi, v, inv);
+      const u32x2 two = result4(v, inv);
+      *reinterpret_cast<u32x2*>(dst + 32 * dt + 8 * g) = two;
+      if (a.out_pack) *reinterpret_cast<u32x2*>(a.out_pack + pack_off(row, first + 32 * dt + 8 * g, a.H * PA_DH)) = two;
     }
-  if (parts > 1 && hi == 0) put_stats(a, parts, part, qh, m_run, l_run);
 }
 
 // ---- 16 columns of one wave over its row's own keys, 32 a step: keys straight from memory into registers (lane's key lane & 15 of each
 // 16, dims 32 j + 8 (lane >> 4) .. +7, the query's the same), values through two wave-private LDS slots.
 JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int split, int kvh, int b, int ct, char* lds) {
   const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-  const int rep = a.H / a.Hkv, ncols = a.S * rep;
+  const int rep = a.rep, ncols = a.S * rep;
   const int c0 = 16 * ct, c = min(c0 + j, ncols - 1);
   const size_t qh = ((size_t)b * a.S + c / rep) * a.H + kvh * rep + c % rep;
   const float scale = 1.4426950408889634f / 11.313708498984761f;
@@ -320,34 +404,28 @@ JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int spli
   }
   l_run = lane_sum32(lane_sum16(l_run));
   if (c0 + j >= ncols) return;
-  const int parts = p.parts(), part = p.ns + split;
+  float* const dst = part_sums(a, p.ns + split, qh) + 4 * g;
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) {
-    const float v[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
-    put_sums(a, part, qh, 16 * dt + 4 * g, v);
-  }
-  if (g == 0) put_stats(a, parts, part, qh, m_run, l_run);
+  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt];
+  if (g == 0) *reinterpret_cast<float2*>(part_stats(a, p.parts(), p.ns + split, qh)) = make_float2(m_run, l_run);
 }
 
 // One launch: workgroups [0, tiles) take 128 columns each, the others a wave per (row, kv head, 16 columns, split) of own keys.
 __global__ void __launch_bounds__(256, 2) prefix_attn_kernel(PrefixAttn a, PrefixPlan p, int tiles, int own_waves) {
   __shared__ __attribute__((aligned(16))) char lds[4 * PA_TILE];
-  const int rep = a.H / a.Hkv, n = a.B / a.G;
+  const int rep = a.rep, n = a.n;
   if ((int)blockIdx.x < tiles) {
+    // (kv heads first: where they are a multiple of the 8 XCDs, all tiles that read the same keys run on one of them, behind one L2)
     int id = blockIdx.x;
-    const int ct = id % p.ct;
-    id /= p.ct;
+    const int kvh = id % a.Hkv;
+    id /= a.Hkv;
     const int part = id % p.ns;
     id /= p.ns;
-    const int kvh = id % a.Hkv, u = id / a.Hkv;
-    if (p.by_row) {
-      const int ncols = a.S * rep;
-      column_tile(a, p, part, kvh, (size_t)u * a.S, ncols, ct, prefix_keys(a, u / n, kvh),
-                  own_keys(a, u, kvh, (min(ncols, (ct + 1) * PA_COLS) - 1) / rep), lds);
-    } else {
-      KeyRange none{};
-      column_tile(a, p, part, kvh, (size_t)u * n * a.S, n * a.S * rep, ct, prefix_keys(a, u, kvh), none, lds);
-    }
+    const int ct = id % p.ct, u = id / p.ct;
+    const int ncols = (p.by_row ? 1 : n) * a.S * rep;
+    KeyRange own = own_keys(a, u, kvh, (min(ncols, (ct + 1) * PA_COLS) - 1) / rep);  // (by a group's number: row u exists too)
+    if (!p.by_row) own.hi = own.lo;
+    column_tile(a, p, part, kvh, (size_t)u * (p.by_row ? 1 : n) * a.S, ncols, ct, prefix_keys(a, p.by_row ? u / n : u, kvh), own, lds);
     return;
   }
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -360,48 +438,78 @@ __global__ void __launch_bounds__(256, 2) prefix_attn_kernel(PrefixAttn a, Prefi
   own_step_columns(a, p, split, id % a.Hkv, id / a.Hkv, ct, lds + w * PA_TILE);
 }
 
-// 32 lanes per (token, head), four of its dims each: the parts join in their order
+// The parts of a (token, head) join in their order: 8 groups of 32 lanes (4 dims each) take every eighth part, so that their loads are
+// under way together, and add up in LDS.
 __global__ void __launch_bounds__(256) prefix_join_kernel(PrefixAttn a, int parts) {
-  const size_t n = (size_t)a.B * a.S * a.H, qh = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (qh >= n) return;
-  const int d = 4 * (threadIdx.x & 31);
-  const float* ml = a.part + n * PA_DH * parts + qh * 2;
+  __shared__ f32x4 so[8][32];
+  __shared__ float sl[8];
+  const size_t n = (size_t)a.B * a.S * a.H, qh = blockIdx.x;
+  const int g = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
+  const float* ml = part_stats(a, parts, 0, qh);
   float m = -INFINITY;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, ml[2 * n * i]);
+  for (int i = threadIdx.x & 31; i < parts; i += 32) m = fmaxf(m, ml[2 * n * i]);
+#pragma unroll
+  for (int j = 1; j < 32; j <<= 1) m = fmaxf(m, __shfl_xor(m, j, 64));
   const float m_use = m == -INFINITY ? 0.f : m;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
-  for (int i = 0; i < parts; ++i) {
+#pragma unroll 4
+  for (int i = g; i < parts; i += 8) {
     const float2 s = *reinterpret_cast<const float2*>(ml + 2 * n * i);
     const float f = __builtin_amdgcn_exp2f(s.x - m_use);
     l += f * s.y;
     o += f * *reinterpret_cast<const f32x4*>(a.part + (n * i + qh) * PA_DH + d);
   }
+  so[g][d >> 2] = o;
+  if (d == 0) sl[g] = l;
+  __syncthreads();
+  if (g) return;
+  const int groups = min(parts, 8);
+  for (int i = 1; i < groups; ++i) {
+    o += so[i][d >> 2];
+    l += sl[i];
+  }
   const float v[4] = {o[0], o[1], o[2], o[3]};
-  put_result(a, qh, d, v, l != 0.f ? 1.f / l : 0.f);
+  const u32x2 two = result4(v, l != 0.f ? 1.f / l : 0.f);
+  *reinterpret_cast<u32x2*>(a.out + qh * PA_DH + d) = two;
+  if (a.out_pack) *reinterpret_cast<u32x2*>(a.out_pack + pack_off((int)(qh / a.H), (int)(qh % a.H) * PA_DH + d, a.H * PA_DH)) = two;
 }
 
 static int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// Which queries share a workgroup, and how the keys are split.
+//
+// A row's own columns go over prefix and own keys together from 96 of them on, else a group's over the prefix with the own keys beside:
+// 16 rows behind 4096 tokens, 8 kv heads, us shared | by row: 16 columns each 30 | 31, 64 41 | 46, 96 59 | 53, 224 106 | 94.
+//
+// Splits: a tile takes 1.15 us where a compute unit has one workgroup and 2.05 where it has two, in rounds of 512; each part's sums are
+// written and read at about 4.5 TB/s, and their join costs a launch. The fewest splits of the least time that makes: 32 rows behind 2048
+// tokens 16.5 us with 12 splits (4: 20.9, 32: 19.1), 200 behind 16384 73.8 with 9 (4: 97), 1000 queries of one row behind 8000 171 with 2
+// (1: 186, 3: 181), 200 queries of 4 rows behind 2000 51 with 1 (2: 65).
 PrefixPlan prefix_attn_plan(int B, int S, int H, int Hkv, int G, int P, int T) {
   PrefixPlan p{};
   const int rep = H / Hkv, n = B / G;
-  const int pre = ceil_div(P, PA_KT), own = ceil_div(T, PA_KT);
   p.by_row = S * rep >= 96;
-  const int cols = p.by_row ? S * rep : n * S * rep;
+  const int cols = (p.by_row ? 1 : n) * S * rep, keys = ceil_div(P, PA_KT) + (p.by_row ? ceil_div(T, PA_KT) : 0);
   p.ct = ceil_div(cols, PA_COLS);
   const long long tiles = (long long)(p.by_row ? B : G) * Hkv * p.ct;
-  const int keys = p.by_row ? pre + own : pre;
-  const long long want = tiles >= 384 ? 1 : (512 + tiles - 1) / tiles;
-  p.ns = (int)(want < 1 ? 1 : want > (keys + 1) / 2 ? (keys + 1) / 2 : want);
-  if (p.ns < 1) p.ns = 1;
-  if (!p.by_row) {
+  auto tiles_time = [&](int ns) {
+    const long long groups = tiles * ns, rest = groups % 512;
+    return ceil_div(keys, ns) * ((double)(groups / 512) * 2.05 + (rest == 0 ? 0. : rest <= 256 ? 1.15 : 2.05));
+  };
+  const double part = 2. * 4 * (PA_DH + 2) * B * S * H / 4.5e6;  // us
+  double best = 1e30;
+  p.ns = 1;
+  for (int ns = 1; ns <= keys && ns <= 256; ++ns) {
+    const double t = tiles_time(ns) + (p.by_row && ns == 1 ? 0. : part * ns + 3.5);
+    if (t < best) best = t, p.ns = ns;
+  }
+  if (!p.by_row) {  // own keys: a wave's step takes about 0.6 us; as long as the prefix's tiles run, or 3
     p.own_ct = ceil_div(S * rep, 16);
-    const long long waves = (long long)B * Hkv * p.own_ct;
-    const int steps = ceil_div(T, PA_STEP);
-    const long long w = waves >= 1024 ? 1 : (1024 + waves - 1) / waves;
-    p.own_ns = (int)(w > (steps + 3) / 4 ? (steps + 3) / 4 : w);
-    if (p.own_ns < 1) p.own_ns = 1;
+    const double steps = ceil_div(T, PA_STEP) * 0.6, beside = tiles_time(p.ns) > 3. ? tiles_time(p.ns) : 3.;
+    const long long waves = (long long)B * Hkv * p.own_ct, most = waves >= 2048 ? 1 : 2048 / waves;
+    const long long want = (long long)(steps / beside) + 1;
+    p.own_ns = (int)(want < most ? want : most);
   }
   return p;
 }
@@ -417,7 +525,7 @@ int prefix_attn(const PrefixAttn& a, const PrefixPlan& p, hipStream_t s) {
   if (parts > 1 && !a.part) return -2;
   const long long tiles = (long long)(p.by_row ? a.B : a.G) * a.Hkv * p.ct * p.ns;
   const long long own_waves = p.by_row ? 0 : (long long)a.B * a.Hkv * p.own_ct * p.own_ns;
-  const long long grid = tiles + (own_waves + 3) / 4, join = ((long long)a.B * a.S * a.H + 7) / 8;
+  const long long grid = tiles + (own_waves + 3) / 4, join = (long long)a.B * a.S * a.H;
   if (grid > 0x7fffffff || own_waves > 0x7ffffff0 || join > 0x7fffffff) return -3;
   prefix_attn_kernel<<<(int)grid, 256, 0, s>>>(a, p, (int)tiles, (int)own_waves);
   hipError_t e = hipGetLastError();

@@ -22,6 +22,7 @@ struct PrefixAttn {
   uint16_t* out_pack;        // optional packed copy (common.h pack_off)
   float* part;               // workspace: prefix_attn_workspace floats
   int B, S, H, Hkv, G, P, T;
+  int rep, n;                // query heads per kv head, rows per prefix
 };
 struct PrefixPlan {
   int by_row;   // column tiles of one row over prefix and own keys, else tiles over a group's rows plus each row's own keys
