@@ -36,6 +36,8 @@ JLA_DEV u32x2 ld_tr(const char* lds, int off) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + off)));
 }
 
+JLA_DEV int own_slot(const PrefixAttn& a) { return a.slot ? a.slot[0] : a.slot0; }
+
 // keys [lo, hi) of one sequence in tiles aligned to its start
 struct KeyRange {
   const bf16_t *k, *v;
@@ -61,7 +63,7 @@ JLA_DEV KeyRange own_keys(const PrefixAttn& a, int b, int kvh, int s_last) {
   r.k = a.ko + b * a.ko_b + kvh * a.ko_h;
   r.v = a.vo + b * a.vo_b + kvh * a.vo_h;
   r.lo = a.kv_start ? max(a.kv_start[b], 0) : 0;
-  r.hi = min(a.slot[0] + s_last + 1, a.T);
+  r.hi = min(own_slot(a) + s_last + 1, a.T);
   r.limit = a.T;
   r.mask = nullptr;
   return r;
@@ -86,7 +88,7 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
   const bool active = c0 < ncols;  // (the wave's; the others help to stage)
   const float scale = 1.4426950408889634f / 11.313708498984761f;
   // a column's slot; those of the wave's first and last columns
-  const int slot = a.slot[0], at_first = slot + min(c0, ncols - 1) / rep, at_last = slot + min(c0 + 31, ncols - 1) / rep;
+  const int slot = own_slot(a), at_first = slot + min(c0, ncols - 1) / rep, at_last = slot + min(c0 + 31, ncols - 1) / rep;
   const int c = min(c0 + col, ncols - 1), at = slot + c / rep;
   const size_t qh = (tok0 + c / rep) * a.H + kvh * rep + c % rep;
   u32x4 qf[8];
@@ -313,7 +315,7 @@ JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int spli
   const size_t qh = ((size_t)b * a.S + c / rep) * a.H + kvh * rep + c % rep;
   const float scale = 1.4426950408889634f / 11.313708498984761f;
   const KeyRange r = own_keys(a, b, kvh, min(c0 + 15, ncols - 1) / rep);
-  const int upto = min(a.slot[0] + c / rep, r.hi - 1);
+  const int upto = min(own_slot(a) + c / rep, r.hi - 1);
   const int n = r.tiles(PA_STEP);
   const int from = (int)((long long)n * split / p.own_ns), to = (int)((long long)n * (split + 1) / p.own_ns);
   u32x4 qf[4];

@@ -13,7 +13,8 @@ struct PrefixAttn {
   const uint16_t *kp, *vp;   // prefix keys and values [G, Hkv, P, 128]; row b reads prefix b / (B / G)
   const uint16_t *ko, *vo;   // own keys and values [B, Hkv, T, 128]
   long long kp_g, kp_h, vp_g, vp_h, ko_b, ko_h, vo_b, vo_h;  // strides in elements (tokens are 128 apart)
-  const int32_t* slot;       // [1]: own slot of a row's first query
+  const int32_t* slot;       // [1]: own slot of a row's first query; null: slot0
+  int slot0;
   const int32_t* prefix_len;    // optional [G]: keys of the prefix (else P)
   const int32_t* prefix_start;  // optional [G]: its first key
   const uint8_t* prefix_mask;   // optional [G, P]
@@ -44,7 +45,8 @@ struct LogitsArgs {
   const int32_t* history;    // optional [B, L]: token ids of each row (row stride ldh), those outside the vocabulary are ignored
   long long ldh;
   int L;
-  const int32_t* length;     // [1]: places of history in use
+  const int32_t* length;     // [1]: places of history in use; null: length0
+  int length0;
   const int32_t* start;      // optional [B]: first of them
   const uint8_t* hmask;      // optional [B, L] (row stride ldm): places that count
   long long ldm;
@@ -63,24 +65,30 @@ struct LogitsArgs {
 int process_logits(const LogitsArgs& a, hipStream_t s);
 
 // ---- cache rows (cache_rows.hip)
-struct RowSpan {             // one tensor of a cache
+struct RowSpan {             // a tensor, or several equal ones (layers) at one distance, of a cache
   uint64_t base;             // address of row 0
   long long row_bytes;       // from a row to the next
+  long long layer_bytes;     // from a layer to the next
   long long run_bytes;       // from a run (a head's tokens) to the next
-  long long runs;            // runs per row
+  long long layers, runs;    // runs: per row and layer
   long long token_bytes;     // bytes of a run per token, or 0: fixed_bytes whatever the tokens
   long long fixed_bytes;
 };
 // Steps (a, b) of a chain run in order, each thread at its own place of every row: b >= 0: row a (ROW_ZERO: zeros, ROW_SAVED: the saved
 // one) goes to row b; b == ROW_SAVED: row a is saved. No chain writes a row that another one reads or writes.
 constexpr int ROW_ZERO = -1, ROW_SAVED = -2;
-constexpr int ROW_STEPS = 400;  // steps of a program that travels as the kernel's argument
-struct RowProgram {
-  int32_t step[2 * ROW_STEPS];
-  uint16_t chain[ROW_STEPS + 1];  // first step of each chain, and the end
+constexpr int ROW_STEPS = 320, ROW_FEW = 32, ROW_SPANS = 2;  // what travels as the kernel's argument
+template <int STEPS>
+struct RowProgramOf {
+  int32_t step[2 * STEPS];
+  uint16_t chain[STEPS + 1];  // first step of each chain, and the end
+  RowSpan src[ROW_SPANS], dst[ROW_SPANS];
 };
-// long_program: [2 * n_steps] steps, then [n_chains + 1] first steps, on the device (programs of more than ROW_STEPS), else null
-int copy_rows(const RowSpan* src, const RowSpan* dst, int spans, const RowProgram& program, const int32_t* long_program,
-              int n_steps, int n_chains, int tokens, long long widest, hipStream_t s);
+using RowProgram = RowProgramOf<ROW_STEPS>;
+using RowProgramFew = RowProgramOf<ROW_FEW>;
+// long_program: [2 * n_steps] steps, then [n_chains + 1] first steps, on the device (programs of more than ROW_STEPS), else null.
+// src, dst: the spans on the device (more than ROW_SPANS), else null. blocks: 16 KiB pieces of the span that has most
+int copy_rows(const RowProgram& program, const int32_t* long_program, const RowSpan* src, const RowSpan* dst, int spans, int n_steps,
+              int n_chains, int tokens, long long blocks, hipStream_t s);
 
 }  // namespace jla

@@ -27,9 +27,7 @@ def _copy_rows(cache, src, dst, tokens, to) -> None:
     tokens = cache.index if tokens is None else int(tokens)
     if not 0 <= tokens <= min(cache.max_length, target.max_length):
         raise ValueError(f"{tokens} tokens of rows of {cache.max_length} and {target.max_length}")
-    src, dst = [int(r) for r in src], [int(r) for r in dst]
-    cache_rows.check_pairs(src, dst, cache.batch_size, target.batch_size)
-    cache_rows.copy_rows(cache.row_layout(), target.row_layout(), src, dst, tokens)
+    cache.row_layout().copy(target.row_layout(), src, dst, tokens)
 
 
 class KVCache:
@@ -53,14 +51,14 @@ class KVCache:
     def row_layout(self) -> cache_rows.RowLayout:
         at = (self.k.data_ptr(), self.v.data_ptr())
         if self._row_layout is None or self._row_layout[0] != at:
-            self._row_layout = at, cache_rows.RowLayout([(x, True) for i in range(self.k.shape[0]) for x in self.layer(i)])
+            self._row_layout = at, cache_rows.RowLayout(self.batch_size, layers=(self.k, self.v))
         return self._row_layout[1]
 
     def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None, to: Optional["KVCache"] = None) -> None:
         """Row ``dst[i]`` becomes row ``src[i]`` (-1: zeros) in every layer, its first ``tokens`` tokens (default: as many as the cache
         holds by its host counter): forks, reordering, moving live rows to the front. Every source is read as it was before the call; a row is
         written once at most. ``to``: the rows written are those of another cache with the same layers (whose slot counter stays as it is).
-        One launch; up to some 400 rows also while a stream is captured, once the caches have copied rows before."""
+        One launch; up to some 300 rows also while a stream is captured, once the caches have copied rows before."""
         _copy_rows(self, src, dst, tokens, to)
 
     def layer(self, i: int):
@@ -299,8 +297,8 @@ class HybridCache:
 
     def row_layout(self) -> cache_rows.RowLayout:
         if self._row_layout is None:
-            held = [(t, True) for t in {id(t): t for d in (self._k, self._v) for t in d.values()}.values()]
-            self._row_layout = cache_rows.RowLayout(held + [(t, False) for d in (self._state, self._conv) for t in d.values()])
+            held = {id(t): t for d in (self._k, self._v) for t in d.values()}.values()
+            self._row_layout = cache_rows.RowLayout(self.batch_size, tokens=held, state=[t for d in (self._state, self._conv) for t in d.values()])
         return self._row_layout
 
     def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None, to: Optional["HybridCache"] = None) -> None:

@@ -1,7 +1,8 @@
 """Ops of serving many continuations of shared prompts (``csrc/serving`` -> ``jax_llama_amd._C_serving``).
 
 Same dispatch rule as the rest of ``ops``: GPU tensors run the hand-written gfx950 kernels (a missing extension raises), CPU
-tensors the PyTorch implementation below. Shapes, types and ranges that the host can see are checked on both.
+tensors the PyTorch implementation below. Shapes, types and ranges that the host can see are checked on both (for the GPU in
+``csrc/serving/bindings.cpp``) and refused with a ValueError.
 
   * ``prefix_attention``: attention of a batch whose rows share prefixes -- continuations of one prompt, or prompts behind a
     common one -- whose keys and values are held and read once;
@@ -15,8 +16,6 @@ import math
 from typing import Optional, Union
 
 import torch
-
-from .slots import slot_tensor as _slot_tensor
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -75,14 +74,20 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     A query with no key gives zeros. What lies at places that no query of the call attends may be anything, NaN included; a value
     that some query attends has to be finite for the queries of its row before it. Keys and values may be views whose heads and rows
     are strided (the tokens of a head follow one another). ``out_packed``: see ``attention``, up to 64 rows."""
-    _need(q.dim() == 4 and k_prefix.dim() == 4 and k_cache.dim() == 4, "prefix_attention takes q [B, S, H, D] and keys [rows, Hkv, tokens, D]")
+    if q.device.type == "cuda":
+        return ext().prefix_attn(q, k_prefix, v_prefix, k_cache, v_cache, slot0, prefix_len, prefix_start, prefix_mask, kv_start, out_packed)
+    return _prefix_attention_cpu(q, k_prefix, v_prefix, k_cache, v_cache, slot0, prefix_len, prefix_start, prefix_mask, kv_start)
+
+
+def _prefix_attention_cpu(q, kp, vp, ko, vo, slot0, prefix_len, prefix_start, prefix_mask, kv_start) -> torch.Tensor:
+    _need(q.dim() == 4 and kp.dim() == 4 and ko.dim() == 4, "prefix_attention takes q [B, S, H, D] and keys [rows, Hkv, tokens, D]")
     b, s, h, d = q.shape
-    g, hkv, p, _ = k_prefix.shape
-    t = k_cache.shape[2]
+    g, hkv, p, _ = kp.shape
+    t = ko.shape[2]
     _need(min(b, s, h, g, hkv, p, t) > 0, "prefix_attention: an axis is empty")
     _need(b % g == 0, f"{b} rows are not a multiple of {g} prefixes")
     _need(h % hkv == 0, f"{h} heads are not a multiple of {hkv} key / value heads")
-    _need(tuple(k_prefix.shape) == tuple(v_prefix.shape) == (g, hkv, p, d) and tuple(k_cache.shape) == tuple(v_cache.shape) == (b, hkv, t, d),
+    _need(tuple(kp.shape) == tuple(vp.shape) == (g, hkv, p, d) and tuple(ko.shape) == tuple(vo.shape) == (b, hkv, t, d),
           f"prefix_attention: keys and values are [{g}, {hkv}, {p}, {d}] of the prefixes and [{b}, {hkv}, {t}, {d}] of the rows")
     _ints(prefix_len, q, g, "prefix_len")
     _ints(prefix_start, q, g, "prefix_start")
@@ -92,19 +97,7 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
               and prefix_mask.device == q.device, f"prefix_mask must be a contiguous uint8 [{g}, {p}] on {q.device}")
     if not torch.is_tensor(slot0):
         _need(0 <= int(slot0) and int(slot0) + s <= t, f"own slots {int(slot0)} .. {int(slot0) + s - 1} lie outside the cache's {t}")
-    if q.device.type != "cuda":
-        return _prefix_attention_cpu(q, k_prefix, v_prefix, k_cache, v_cache, slot0, prefix_len, prefix_start, prefix_mask, kv_start)
-    _need(d == HEAD_DIM, f"prefix_attention: heads of {HEAD_DIM} on the GPU, not {d}")
-    out = torch.empty(b * s, h * d, dtype=BF16, device=q.device)
-    ext().prefix_attn(q, k_prefix, v_prefix, k_cache, v_cache, _slot_tensor(slot0, q.device), prefix_len, prefix_start, prefix_mask, kv_start,
-                      out, out_packed)
-    return out
-
-
-def _prefix_attention_cpu(q, kp, vp, ko, vo, slot0, prefix_len, prefix_start, prefix_mask, kv_start) -> torch.Tensor:
-    b, s, h, d = q.shape
-    g, hkv, p, _ = kp.shape
-    n, rep, t = b // g, h // hkv, ko.shape[2]
+    n, rep = b // g, h // hkv
     slot = int(slot0.reshape(-1)[0]) if torch.is_tensor(slot0) else int(slot0)
     place = torch.arange(p)[None, :]
     ok_p = torch.ones(g, p, dtype=torch.bool)
@@ -176,6 +169,28 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     (``pack_allowed``), one mask for all, one per row, or row ``allowed_rows[b]`` of them (int32 ``[B]``; an index outside the masks allows
     everything). ``vocab_start``: token id of column 0 (a vocabulary shard); ``bias`` has the shard's columns, ``allowed`` all ids.
     ``out``: ``logits`` itself (in place; without bias and mask only the history's tokens are touched) or another tensor."""
+    if logits.device.type == "cuda":
+        return ext().process_logits(logits, out, history, length, start, history_mask, prompt_len, vocab_start, repetition_penalty,
+                                    presence_penalty, frequency_penalty, bias, allowed, allowed_rows)
+    return _process_logits_cpu(logits, history, length, start, history_mask, prompt_len, vocab_start, repetition_penalty, presence_penalty,
+                               frequency_penalty, bias, allowed, allowed_rows, out)
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def ends(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
+def _process_logits_cpu(logits, history, length, start, history_mask, prompt_len, vocab_start, repetition_penalty, presence_penalty,
+                        frequency_penalty, bias, allowed, allowed_rows, out) -> torch.Tensor:
     _need(logits.dim() == 2 and logits.dtype == F32, "process_logits takes fp32 logits [B, V]")
     b, v = logits.shape
     _need(v <= 1 or logits.stride(1) == 1, "logits must have unit inner stride")
@@ -221,29 +236,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
         _need(_same(out, logits) or not _overlap(out, logits), "out is the logits or shares nothing with them")
     if b > 1:  # rows of one output apart
         _need(out.stride(0) >= v, "rows of out overlap")
-    if logits.device.type != "cuda":
-        return _process_logits_cpu(logits, history, length, start, history_mask, prompt_len, vocab_start, repetition_penalty, presence_penalty,
-                                   frequency_penalty, bias, allowed, allowed_rows, out)
-    ext().process_logits(logits, out, history, None if history is None else _slot_tensor(length, logits.device), start, history_mask,
-                         int(prompt_len), int(vocab_start), repetition_penalty, presence_penalty, frequency_penalty, bias, allowed, allowed_rows)
-    return out
-
-
-def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    def ends(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
-    if not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = ends(a), ends(b)
-    return a0 < b1 and b0 < a1
-
-
-def _process_logits_cpu(x, history, length, start, history_mask, prompt_len, vocab_start, rep, pres, freq, bias, allowed, allowed_rows, out):
-    b, v = x.shape
+    x, rep, pres, freq = logits, repetition_penalty, presence_penalty, frequency_penalty
     y = x.clone()
 
     def col(val):

@@ -201,3 +201,5 @@ def test_copy_rows_refusals():
         hy.copy_rows([0], [1], tokens=1, to=HybridCache(SPECS[:3], 4, 6, "cpu"))
     with pytest.raises(ValueError):
         kv.copy_rows([0], [1], tokens=5, to=KVCache(2, 4, 2, 4, 16, "cpu"))
+    with pytest.raises(ValueError):  # as many bytes, other numbers
+        kv.copy_rows([0], [1], tokens=1, to=KVCache(2, 4, 2, 6, 8, "cpu", torch.float32))

@@ -146,12 +146,19 @@ def test_prefix_attention_refusals_gpu():
     q, kp, vp, ko, vo = (x.to(DEV) for x in inputs(2, 1, 1, 4, 2, 16, 8, unused=0.0))
     for bad in ((q[..., :64].contiguous(), kp[..., :64].contiguous(), vp[..., :64].contiguous(), ko[..., :64].contiguous(), vo[..., :64].contiguous()),
                 (q, kp.cpu(), vp, ko, vo), (q.float(), kp, vp, ko, vo), (q, kp.float(), vp, ko, vo), (q.repeat(1, 1, 1, 2)[..., :128], kp, vp, ko, vo)):
-        with pytest.raises((ValueError, RuntimeError)):
+        with pytest.raises(ValueError):
             ops.prefix_attention(*bad, 0)
+    for kw in (dict(prefix_len=torch.ones(2, dtype=I32, device=DEV)), dict(prefix_start=torch.ones(1, device=DEV)), dict(kv_start=torch.ones(1, dtype=I32, device=DEV)),
+               dict(prefix_mask=torch.ones(1, 15, dtype=torch.uint8, device=DEV)), dict(prefix_len=torch.ones(1, dtype=I32))):
+        with pytest.raises(ValueError):
+            ops.prefix_attention(q, kp, vp, ko, vo, 0, **kw)
+    for slot in (8, -1):
+        with pytest.raises(ValueError):
+            ops.prefix_attention(q, kp, vp, ko, vo, slot)
     odd = torch.zeros(1, 2, 16 * 128 + 8, dtype=BF16, device=DEV)
-    with pytest.raises((ValueError, RuntimeError)):  # tokens that do not follow one another
+    with pytest.raises(ValueError):  # tokens that do not follow one another
         ops.prefix_attention(q, kp.transpose(1, 2).contiguous().transpose(1, 2), vp, ko, vo, 0)
-    with pytest.raises((ValueError, RuntimeError)):  # not at a multiple of 16 bytes
+    with pytest.raises(ValueError):  # not at a multiple of 16 bytes
         ops.prefix_attention(q, odd[:, :, 1:16 * 128 + 1].unflatten(2, (16, 128)), vp, ko, vo, 0)
 
 
@@ -290,10 +297,45 @@ def test_copy_rows_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(t, w) for (t, _, _), w in zip(cache_tensors(cache), want))
-    fresh = KVCache(1, 2, 1, 2, 128, DEV)
+    fresh = HybridCache(SPECS, 4, 6, DEV)
     with pytest.raises(RuntimeError):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             fresh.copy_rows([0], [1], tokens=1)
+
+
+def test_copy_rows_refusals_gpu():
+    kv, hy = KVCache(2, 4, 2, 6, 128, DEV), HybridCache(SPECS, 4, 6, DEV)
+    for cache in (kv, hy):
+        for src, dst, kw in (([0], [4], {}), ([4], [0], {}), ([-2], [0], {}), ([0], [-1], {}), ([0, 1], [2, 2], {}), ([0, 1], [2], {}),
+                             ([0], [1], dict(tokens=7)), ([0], [1], dict(tokens=-1))):
+            with pytest.raises(ValueError):
+                cache.copy_rows(src, dst, **kw)
+    for other in (hy, KVCache(2, 4, 3, 6, 128, DEV), KVCache(3, 4, 2, 6, 128, DEV), KVCache(2, 4, 2, 6, 64, DEV, torch.float32)):
+        with pytest.raises(ValueError):
+            kv.copy_rows([0], [1], tokens=1, to=other)
+
+
+def test_process_logits_refusals_gpu():
+    x, h = torch.randn(2, 40, device=DEV), torch.zeros(2, 5, dtype=I32, device=DEV)
+    words = torch.zeros(3, 2, dtype=I32, device=DEV)
+    ok = dict(presence_penalty=0.1, history=h, length=1)
+    bad = [dict(repetition_penalty=1.2), {**ok, "repetition_penalty": 0.0}, {**ok, "presence_penalty": float("inf")}, dict(presence_penalty=0.1, history=h),
+           {**ok, "length": 6}, {**ok, "length": -1}, {**ok, "history": h[:1]}, {**ok, "history": h.long()}, {**ok, "history": h.cpu()},
+           {**ok, "frequency_penalty": torch.zeros(3, device=DEV)}, {**ok, "start": torch.zeros(3, dtype=I32, device=DEV)}, {**ok, "prompt_len": -1},
+           {**ok, "history_mask": torch.ones(2, 4, dtype=torch.uint8, device=DEV)}, dict(bias=torch.zeros(39, device=DEV)), dict(bias=torch.zeros(40)),
+           dict(bias=torch.zeros(1, 40, device=DEV)), dict(bias=torch.zeros(40, dtype=torch.float64, device=DEV)), dict(allowed=words[:, :1]),
+           dict(allowed=words), dict(allowed=words.long()), dict(allowed_rows=torch.zeros(2, dtype=I32, device=DEV)),
+           dict(allowed=words[:1], vocab_start=30), dict(vocab_start=-1), dict(out=torch.zeros(2, 41, device=DEV)), dict(out=torch.zeros(2, 40)),
+           dict(out=torch.zeros(1, 40, device=DEV).expand(2, 40))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.process_logits(x, **kw)
+    for other in (x.to(BF16), x[0], x.t()):
+        with pytest.raises(ValueError):
+            ops.process_logits(other)
+    both = torch.zeros(81, device=DEV)
+    with pytest.raises(ValueError):
+        ops.process_logits(both[:80].view(2, 40), out=both[1:].view(2, 40))
 
 
 # ---------------------------------------------------------------------------------- together
