@@ -339,6 +339,10 @@ struct RowLayout {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefix_attn", &prefix_attn, py::arg("q"), py::arg("kp"), py::arg("vp"), py::arg("ko"), py::arg("vo"), py::arg("slot"),
         py::arg("prefix_len"), py::arg("prefix_start"), py::arg("prefix_mask"), py::arg("kv_start"), py::arg("out_pack"));
+  m.def("prefix_plan", [](int b, int s, int h, int hkv, int g, int p, int t) {
+    const jla::PrefixPlan plan = jla::prefix_attn_plan(b, s, h, hkv, g, p, t);
+    return std::string(plan.brief ? "short" : plan.by_row ? "row" : "group") + (!plan.brief && plan.parts() > 1 ? "+join" : "");
+  });
   m.def("process_logits", &process_logits, py::arg("x"), py::arg("out"), py::arg("history"), py::arg("length"), py::arg("start"),
         py::arg("history_mask"), py::arg("prompt_len"), py::arg("vocab_start"), py::arg("repetition"), py::arg("presence"),
         py::arg("frequency"), py::arg("bias"), py::arg("allowed"), py::arg("allowed_rows"));

@@ -306,48 +306,57 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
     }
 }
 
-// ---- 16 columns of one wave over its row's own keys, 32 a step: keys straight from memory into registers (lane's key lane & 15 of each
-// 16, dims 32 j + 8 (lane >> 4) .. +7, the query's the same), values through two wave-private LDS slots.
-JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int split, int kvh, int b, int ct, char* lds) {
+// ---- 16 columns of one row and one wave, 32 keys a step: keys straight from memory into registers (lane's key lane & 15 of each 16, dims
+// 32 j + 8 (lane >> 4) .. +7, the query's the same), values through two wave-private LDS slots. Steps [from, to) of the prefix's keys (where
+// there are some) and the row's own after them. Lane (g, j) is left with dims 16 dt + 4 g .. + 3 of column j in o[dt].
+struct WaveSums {
+  f32x4 o[8];
+  float m, l;
+};
+constexpr int PA_WAVE_LDS = 2 * PA_STEP * PA_DH * 2;
+
+JLA_DEV void wave_columns(WaveSums& st, const PrefixAttn& a, size_t qh, int upto, const KeyRange& pre, const KeyRange& own, int from, int to, char* lds) {
   const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-  const int rep = a.rep, ncols = a.S * rep;
-  const int c0 = 16 * ct, c = min(c0 + j, ncols - 1);
-  const size_t qh = ((size_t)b * a.S + c / rep) * a.H + kvh * rep + c % rep;
   const float scale = 1.4426950408889634f / 11.313708498984761f;
-  const KeyRange r = own_keys(a, b, kvh, min(c0 + 15, ncols - 1) / rep);
-  const int upto = min(own_slot(a) + c / rep, r.hi - 1);
-  const int n = r.tiles(PA_STEP);
-  const int from = (int)((long long)n * split / p.own_ns), to = (int)((long long)n * (split + 1) / p.own_ns);
+  const int n_pre = pre.tiles(PA_STEP);
   u32x4 qf[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const u32x4*>(a.q + qh * PA_DH + 32 * i + 8 * g);
-  f32x4 o[8];
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.f;
+  for (int dt = 0; dt < 8; ++dt) st.o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  st.m = -INFINITY;
+  st.l = 0.f;
   u32x4 kr[2][8];
-  auto issue = [&](int i, u32x4 (&k)[8], char* vd) {
-    const int t0 = r.first(PA_STEP) + i * PA_STEP;
+  uint32_t kept[2];  // a bit for each of a step's keys that the range and the mask leave
+  auto issue = [&](int i, u32x4 (&k)[8], uint32_t& bits, char* vd) {
+    const bool is_own = i >= n_pre;
+    const int t0 = is_own ? own.first(PA_STEP) + (i - n_pre) * PA_STEP : pre.first(PA_STEP) + i * PA_STEP;
+    const int lo = is_own ? own.lo : pre.lo, hi = is_own ? own.hi : pre.hi, last = (is_own ? own.limit : pre.limit) - 1;
+    const bf16_t* const kp = is_own ? own.k : pre.k;
+    const bf16_t* const vp = is_own ? own.v : pre.v;
+    const uint8_t* const mask = is_own ? nullptr : pre.mask;
+    bits = ~0u;
+    if (t0 < lo || t0 + PA_STEP > hi || mask) {
+      const int key = t0 + (lane & 31);
+      bits = (uint32_t)__ballot(key >= lo && key < hi && (!mask || mask[min(key, last)]));
+    }
 #pragma unroll
     for (int bi = 0; bi < 8; ++bi) {
       const int row = 4 * bi + g, ch = j ^ (((row & 3) << 2) | ((row >> 2) & 3));
-      glds16_asm(r.v + (size_t)min(t0 + row, r.limit - 1) * PA_DH + 8 * ch, vd + 1024 * bi);
+      glds16_asm(vp + (size_t)t0 * PA_DH, 256 * min(row, last - t0) + 16 * ch, vd + 1024 * bi);
     }
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk) {
+      const bf16_t* const at = kp + (size_t)min(t0 + 16 * kk + j, last) * PA_DH + 8 * g;
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4)
-        k[4 * kk + i4] = *reinterpret_cast<const u32x4*>(r.k + (size_t)min(t0 + 16 * kk + j, r.limit - 1) * PA_DH + 32 * i4 + 8 * g);
+      for (int i4 = 0; i4 < 4; ++i4) k[4 * kk + i4] = *reinterpret_cast<const u32x4*>(at + 32 * i4);
+    }
   };
-  auto compute = [&](int i, const u32x4 (&k)[8], char* vt) {
-    const int t0 = r.first(PA_STEP) + i * PA_STEP;
-    const bool edge = t0 < r.lo || t0 + PA_STEP > r.hi;
-    if (edge) {
+  auto compute = [&](int i, const u32x4 (&k)[8], uint32_t bits, char* vt) {
+    if (bits != ~0u) {  // values of keys that nobody attends may be anything: 0 x NaN would not be 0
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int row = 4 * q + g, key = t0 + row;
-        if (key < r.lo || key >= r.hi) *reinterpret_cast<u32x4*>(vt + 256 * row + 16 * j) = u32x4{0u, 0u, 0u, 0u};
-      }
+      for (int q = 0; q < 8; ++q)
+        if (!(bits >> (4 * q + g) & 1)) *reinterpret_cast<u32x4*>(vt + 1024 * q + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
       __builtin_amdgcn_wave_barrier();
     }
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
@@ -356,29 +365,32 @@ JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int spli
       s[0] = mfma16x16x32(k[i4], qf[i4], s[0]);
       s[1] = mfma16x16x32(k[4 + i4], qf[i4], s[1]);
     }
-    float sc[8];  // keys t0 + 4 g + e, and + 16
-    float most = -INFINITY;
+    if (i >= n_pre) {  // a column's own keys end at its slot
+      const int n = upto + 1 - (own.first(PA_STEP) + (i - n_pre) * PA_STEP);
+      bits &= n >= PA_STEP ? ~0u : n > 0 ? (1u << n) - 1 : 0u;
+    }
+    bits >>= 4 * g;  // score e is key 16 (e >> 2) + 4 g + (e & 3) of the step
+    float sc[8], most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int key = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
-      sc[e] = key >= r.lo && key <= upto ? s[e >> 2][e & 3] * scale : -INFINITY;
+      sc[e] = bits >> (16 * (e >> 2) + (e & 3)) & 1 ? s[e >> 2][e & 3] * scale : -INFINITY;
       most = fmaxf(most, sc[e]);
     }
     most = lane_max32(lane_max16(most));
-    if (__ballot(most > m_run + 8.f)) {
-      const float m_new = fmaxf(m_run, most);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
-      l_run *= alpha;
-      m_run = m_new;
+    if (__ballot(most > st.m + 8.f)) {
+      const float m_new = fmaxf(st.m, most);
+      const float alpha = __builtin_amdgcn_exp2f(st.m - (m_new == -INFINITY ? 0.f : m_new));
+      st.l *= alpha;
+      st.m = m_new;
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) o[dt] *= alpha;
+      for (int dt = 0; dt < 8; ++dt) st.o[dt] *= alpha;
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    const float m_use = st.m == -INFINITY ? 0.f : st.m;
     float e[8];
 #pragma unroll
     for (int i8 = 0; i8 < 8; ++i8) {
       e[i8] = __builtin_amdgcn_exp2f(sc[i8] - m_use);
-      l_run += e[i8];
+      st.l += e[i8];
     }
     const u32x4 pf = pack8(e);
     const int row = 4 * g + (j >> 2), pp = lane & 3;
@@ -386,30 +398,89 @@ JLA_DEV void own_step_columns(const PrefixAttn& a, const PrefixPlan& p, int spli
     for (int dt = 0; dt < 8; ++dt) {
       const int ch = 2 * dt + (pp >> 1);
       const u32x2 lo4 = ld_tr(vt, pa_off(row, ch) + 8 * (pp & 1)), hi4 = ld_tr(vt, pa_off(row + 16, ch) + 8 * (pp & 1));
-      o[dt] = mfma16x16x32(u32x4{lo4[0], lo4[1], hi4[0], hi4[1]}, pf, o[dt]);
+      st.o[dt] = mfma16x16x32(u32x4{lo4[0], lo4[1], hi4[0], hi4[1]}, pf, st.o[dt]);
     }
   };
   char* const slot_a = lds;
   char* const slot_b = lds + PA_STEP * PA_DH * 2;
-  if (from < to) issue(from, kr[0], slot_a);
+  if (from < to) issue(from, kr[0], kept[0], slot_a);
   for (int i = from; i < to; i += 2) {
     wait_vmcnt<0>();
-    if (i + 1 < to) issue(i + 1, kr[1], slot_b);
-    compute(i, kr[0], slot_a);
+    if (i + 1 < to) issue(i + 1, kr[1], kept[1], slot_b);
+    compute(i, kr[0], kept[0], slot_a);
     if (i + 1 < to) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // slot a is read: it may be filled again
       wait_vmcnt<0>();
-      if (i + 2 < to) issue(i + 2, kr[0], slot_a);
-      compute(i + 1, kr[1], slot_b);
+      if (i + 2 < to) issue(i + 2, kr[0], kept[0], slot_a);
+      compute(i + 1, kr[1], kept[1], slot_b);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   }
-  l_run = lane_sum32(lane_sum16(l_run));
+  st.l = lane_sum32(lane_sum16(st.l));
+}
+
+// a wave's split of a row's own keys, beside the prefix's tiles
+JLA_DEV void own_part(const PrefixAttn& a, const PrefixPlan& p, int split, int kvh, int b, int ct, char* lds) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+  const int ncols = a.S * a.rep, c0 = 16 * ct, c = min(c0 + j, ncols - 1);
+  const size_t qh = ((size_t)b * a.S + c / a.rep) * a.H + kvh * a.rep + c % a.rep;
+  const KeyRange own = own_keys(a, b, kvh, min(c0 + 15, ncols - 1) / a.rep);
+  const int n = own.tiles(PA_STEP);
+  WaveSums st;
+  wave_columns(st, a, qh, own_slot(a) + c / a.rep, KeyRange{}, own, (int)((long long)n * split / p.own_ns), (int)((long long)n * (split + 1) / p.own_ns), lds);
   if (c0 + j >= ncols) return;
   float* const dst = part_sums(a, p.ns + split, qh) + 4 * g;
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt];
-  if (g == 0) *reinterpret_cast<float2*>(part_stats(a, p.parts(), p.ns + split, qh)) = make_float2(m_run, l_run);
+  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = st.o[dt];
+  if (g == 0) *reinterpret_cast<float2*>(part_stats(a, p.parts(), p.ns + split, qh)) = make_float2(st.m, st.l);
+}
+
+// Short prefixes: one launch. A workgroup of eight waves takes 16 columns of a (row, kv head) over prefix and own keys, each wave an eighth of
+// their steps; the waves' parts join in LDS.
+constexpr int PS_WAVES = 8, PS_LDS = PS_WAVES * PA_WAVE_LDS;
+
+__global__ void __launch_bounds__(64 * PS_WAVES, 2) prefix_short_kernel(PrefixAttn a, PrefixPlan p) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, j = lane & 15;
+  int id = blockIdx.x;
+  const int kvh = id % a.Hkv;
+  id /= a.Hkv;
+  const int ct = id % p.own_ct, b = id / p.own_ct;
+  const int ncols = a.S * a.rep, c0 = 16 * ct, c = min(c0 + j, ncols - 1);
+  const size_t row0 = (size_t)b * a.S;
+  const KeyRange pre = prefix_keys(a, b / a.n, kvh), own = own_keys(a, b, kvh, min(c0 + 15, ncols - 1) / a.rep);
+  const int n = pre.tiles(PA_STEP) + own.tiles(PA_STEP);
+  WaveSums st;
+  wave_columns(st, a, (row0 + c / a.rep) * a.H + kvh * a.rep + c % a.rep, own_slot(a) + c / a.rep, pre, own, n * w / PS_WAVES, n * (w + 1) / PS_WAVES,
+               lds + w * PA_WAVE_LDS);
+  // [32 chunks of 4 dims][16 columns and one for the banks] sums, then the statistics, in each wave's share
+  auto sums = [&](int wave) { return reinterpret_cast<f32x4*>(lds + wave * PA_WAVE_LDS); };
+  auto stats = [&](int wave) { return reinterpret_cast<float2*>(lds + wave * PA_WAVE_LDS + 32 * 17 * 16); };
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) sums(w)[(4 * dt + g) * 17 + j] = st.o[dt];
+  if (g == 0) stats(w)[j] = make_float2(st.m, st.l);
+  __syncthreads();
+  const int oc = tid >> 5, q = tid & 31;  // its column and chunk
+  if (c0 + oc >= ncols) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PS_WAVES; ++i) m = fmaxf(m, stats(i)[oc].x);
+  const float m_use = m == -INFINITY ? 0.f : m;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PS_WAVES; ++i) {
+    const float2 s = stats(i)[oc];
+    const float f = __builtin_amdgcn_exp2f(s.x - m_use);
+    l += f * s.y;
+    o += f * sums(i)[q * 17 + oc];
+  }
+  const float v[4] = {o[0], o[1], o[2], o[3]};
+  const u32x2 two = result4(v, l != 0.f ? 1.f / l : 0.f);
+  const size_t row = row0 + (c0 + oc) / a.rep;
+  const int d = (kvh * a.rep + (c0 + oc) % a.rep) * PA_DH + 4 * q;
+  *reinterpret_cast<u32x2*>(a.out + row * a.H * PA_DH + d) = two;
+  if (a.out_pack) *reinterpret_cast<u32x2*>(a.out_pack + pack_off((int)row, d, a.H * PA_DH)) = two;
 }
 
 // One launch: workgroups [0, tiles) take 128 columns each, the others a wave per (row, kv head, 16 columns, split) of own keys.
@@ -437,7 +508,7 @@ __global__ void __launch_bounds__(256, 2) prefix_attn_kernel(PrefixAttn a, Prefi
   id /= p.own_ct;
   const int split = id % p.own_ns;
   id /= p.own_ns;
-  own_step_columns(a, p, split, id % a.Hkv, id / a.Hkv, ct, lds + w * PA_TILE);
+  own_part(a, p, split, id % a.Hkv, id / a.Hkv, ct, lds + w * PA_WAVE_LDS);
 }
 
 // The parts of a (token, head) join in their order: 8 groups of 32 lanes (4 dims each) take every eighth part, so that their loads are
@@ -513,16 +584,30 @@ PrefixPlan prefix_attn_plan(int B, int S, int H, int Hkv, int G, int P, int T) {
     const long long want = (long long)(steps / beside) + 1;
     p.own_ns = (int)(want < most ? want : most);
   }
+  // Short ones in one launch, 16 columns a workgroup: a step of its eight waves takes about 2 us (128 KiB through one compute unit), against 0.9
+  // us more for the two launches: 2 rows behind 130 tokens 5.5 us (8.3), 32 behind 250 7.5 (11.8), 8 behind 700 11.4 (9.8), 64 behind 250
+  // 13.0 (12.9).
+  const int rows_ct = ceil_div(S * rep, 16), steps = ceil_div(ceil_div(P, PA_STEP) + ceil_div(T, PA_STEP), PS_WAVES);
+  const double rounds = (double)(((long long)B * Hkv * rows_ct + 255) / 256);
+  if (rounds * steps * (rounds > 1. ? 2.4 : 2.) < best + 0.9) p.brief = 1, p.own_ct = rows_ct;
   return p;
 }
 
 long long prefix_attn_workspace(const PrefixPlan& p, int B, int S, int H) {
-  return p.parts() > 1 ? (long long)p.parts() * B * S * H * (PA_DH + 2) : 0;
+  return !p.brief && p.parts() > 1 ? (long long)p.parts() * B * S * H * (PA_DH + 2) : 0;
 }
 
 int prefix_attn(const PrefixAttn& a, const PrefixPlan& p, hipStream_t s) {
   if (a.B <= 0 || a.S <= 0) return 0;
   if (a.H % a.Hkv || a.G <= 0 || a.B % a.G || a.P < 1 || a.T < 1) return -1;
+  if (p.brief) {
+    static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_short_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PS_LDS);
+    if (room != hipSuccess) return (int)room;
+    const long long items = (long long)a.B * a.Hkv * p.own_ct;
+    if (items > 0x7fffffff) return -3;
+    prefix_short_kernel<<<(int)items, 64 * PS_WAVES, PS_LDS, s>>>(a, p);
+    return (int)hipGetLastError();
+  }
   const int parts = p.parts();
   if (parts > 1 && !a.part) return -2;
   const long long tiles = (long long)(p.by_row ? a.B : a.G) * a.Hkv * p.ct * p.ns;

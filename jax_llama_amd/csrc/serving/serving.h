@@ -29,6 +29,7 @@ struct PrefixPlan {
   int by_row;   // column tiles of one row over prefix and own keys, else tiles over a group's rows plus each row's own keys
   int ct;       // tiles of 128 columns per (group or row, kv head)
   int ns;       // splits of their keys
+  int brief;    // prefix_short_kernel; the others are not looked at but own_ct
   int own_ct;   // not by_row: tiles of 16 columns per (row, kv head)
   int own_ns;   // and splits of the own keys
   __host__ __device__ int parts() const { return ns + (by_row ? 0 : own_ns); }

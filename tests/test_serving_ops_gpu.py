@@ -6,6 +6,7 @@ import torch
 import oracle_serving as oracle
 from jax_llama_amd import ops
 from jax_llama_amd.models.kv_cache import HybridCache, KVCache
+from jax_llama_amd.ops import serving
 from test_serving_ops import SPECS, cache_tensors
 
 pytestmark = pytest.mark.gpu
@@ -31,21 +32,30 @@ def close(got, want, bound):
     assert bool((err <= bound).all()), f"largest excess {float((err - bound).max()):.3e}, largest error {float(err.max()):.3e}"
 
 
-@pytest.mark.parametrize("b,g,s,h,hkv,p,t,slot", [
-    (1, 1, 1, 1, 1, 1, 1, 0),          # one key each
-    (2, 1, 1, 8, 2, 63, 5, 3),
-    (3, 3, 1, 4, 4, 64, 40, 31),       # every row its own prefix
-    (6, 2, 1, 10, 2, 65, 70, 63),      # five query heads per kv head
-    (40, 1, 1, 8, 1, 130, 33, 32),     # 320 columns
-    (33, 1, 1, 16, 1, 300, 3, 1),      # 16 query heads per kv head
-    (4, 2, 2, 6, 2, 200, 130, 100),    # two queries a row
-    (5, 1, 7, 9, 3, 129, 20, 9),       # 21 columns of own keys
-    (2, 2, 33, 8, 2, 70, 40, 4),       # tiles of one row over both
-    (3, 1, 130, 4, 2, 257, 200, 66),
-    (1, 1, 96, 1, 1, 1000, 96, 0),
-    (2, 1, 1, 4, 1, 4100, 1200, 1111),
-])
-def test_prefix_attention(b, g, s, h, hkv, p, t, slot):
+SHAPES = [  # and the way they go (csrc/serving/prefix_attn.hip prefix_attn_plan)
+    (1, 1, 1, 1, 1, 1, 1, 0, "short"),              # one key each
+    (2, 1, 1, 8, 2, 63, 5, 3, "short"),
+    (3, 3, 1, 4, 4, 64, 40, 31, "short"),           # every row its own prefix
+    (6, 2, 1, 10, 2, 65, 70, 63, "short"),          # five query heads per kv head
+    (40, 1, 1, 8, 1, 130, 33, 32, "short"),
+    (33, 1, 1, 16, 1, 300, 3, 1, "short"),          # 16 query heads per kv head
+    (5, 1, 7, 9, 3, 129, 20, 9, "short"),           # 21 columns
+    (2, 2, 33, 8, 2, 70, 40, 4, "short"),
+    (40, 1, 1, 8, 1, 2000, 33, 32, "group+join"),   # 320 columns
+    (4, 2, 2, 6, 2, 2200, 130, 100, "group+join"),  # two queries a row
+    (9, 3, 1, 6, 2, 1025, 300, 290, "group+join"),
+    (2, 1, 1, 4, 1, 4100, 1200, 1111, "group+join"),
+    (70, 7, 3, 20, 4, 700, 40, 8, "group+join"),    # 5 query heads, 150 columns a prefix, 15 of own keys
+    (3, 1, 130, 4, 2, 1257, 200, 66, "row+join"),   # tiles of one row over both
+    (1, 1, 96, 1, 1, 1000, 96, 0, "row+join"),
+    (64, 2, 60, 8, 4, 500, 80, 20, "row"),          # 120 columns a row, one part
+    (13, 1, 97, 12, 4, 640, 130, 33, "row"),        # 291
+]
+
+
+@pytest.mark.parametrize("b,g,s,h,hkv,p,t,slot,way", SHAPES)
+def test_prefix_attention(b, g, s, h, hkv, p, t, slot, way):
+    assert serving.ext().prefix_plan(b, s, h, hkv, g, p, t) == way
     args = inputs(b, g, s, h, hkv, p, t, slot=slot)
     want, bound = oracle.prefix_attention(*args, slot)
     gpu = [x.to(DEV) for x in args]
@@ -54,8 +64,12 @@ def test_prefix_attention(b, g, s, h, hkv, p, t, slot):
     assert torch.equal(got, ops.prefix_attention(*gpu, torch.tensor([slot], dtype=I32, device=DEV)))
 
 
-@pytest.mark.parametrize("b,g,s,h,hkv,p,t,slot", [(8, 4, 1, 4, 2, 150, 70, 60), (6, 3, 3, 4, 1, 70, 40, 33), (6, 3, 40, 3, 1, 200, 90, 20)])
-def test_prefix_attention_masks(b, g, s, h, hkv, p, t, slot):
+@pytest.mark.parametrize("b,g,s,h,hkv,p,t,slot,way", [
+    (8, 4, 1, 4, 2, 150, 70, 60, "short"), (6, 3, 3, 4, 1, 70, 40, 33, "short"), (6, 3, 40, 3, 1, 200, 90, 20, "short"),
+    (8, 4, 1, 8, 2, 1900, 70, 60, "group+join"), (6, 3, 5, 4, 2, 1500, 40, 33, "group+join"), (6, 3, 50, 4, 1, 1100, 190, 20, "row+join"),
+    (60, 3, 50, 8, 4, 600, 90, 20, "row")])
+def test_prefix_attention_masks(b, g, s, h, hkv, p, t, slot, way):
+    assert serving.ext().prefix_plan(b, s, h, hkv, g, p, t) == way
     args = inputs(b, g, s, h, hkv, p, t, slot=slot)
     kw = dict(prefix_len=torch.randint(p // 2, p + 1, (g,), dtype=I32), prefix_start=torch.randint(0, p // 3, (g,), dtype=I32),
               prefix_mask=(torch.rand(g, p) < 0.6).to(torch.uint8), kv_start=torch.randint(0, slot + 1, (b,), dtype=I32))
@@ -86,16 +100,18 @@ def test_prefix_attention_masks(b, g, s, h, hkv, p, t, slot):
         close(ops.prefix_attention(*(x.to(DEV) for x in (q, kp, vp, ko, vo)), slot, **dev(given)), want, bound)
 
 
-def test_prefix_attention_large_scores_and_prefix_alone():
+@pytest.mark.parametrize("p", [700, 5000])
+def test_prefix_attention_large_scores(p):
     """Scores of some hundreds, ascending along the keys (the maximum moves all the time)."""
-    q, kp, vp, ko, vo = inputs(3, 1, 1, 4, 2, 700, 8, slot=2)
-    kp = (kp.float() * torch.linspace(0.1, 12, 700)[None, None, :, None]).to(BF16)
+    q, kp, vp, ko, vo = inputs(3, 1, 1, 4, 2, p, 8, slot=2)
+    kp = (kp.float() * torch.linspace(0.1, 12, p)[None, None, :, None]).to(BF16)
     want, bound = oracle.prefix_attention(q, kp, vp, ko, vo, 2)
     close(ops.prefix_attention(*(x.to(DEV) for x in (q, kp, vp, ko, vo)), 2), want, bound)
 
 
-def test_prefix_attention_views_streams_and_packed():
-    q, kp, vp, ko, vo = inputs(12, 2, 1, 8, 2, 100, 30, unused=0.0, slot=20)
+@pytest.mark.parametrize("p", [100, 2500])
+def test_prefix_attention_views_streams_and_packed(p):
+    q, kp, vp, ko, vo = inputs(12, 2, 1, 8, 2, p, 30, unused=0.0, slot=20)
     want, bound = oracle.prefix_attention(q, kp, vp, ko, vo, 20)
     wide = [torch.full((x.shape[0] + 1, x.shape[1] + 2, x.shape[2] + 5, 128), float("nan"), dtype=BF16, device=DEV) for x in (kp, vp, ko, vo)]
     views = []
@@ -116,9 +132,10 @@ def test_prefix_attention_views_streams_and_packed():
     assert torch.equal(rows, got.view(torch.int16))
 
 
-def test_prefix_attention_graph():
+@pytest.mark.parametrize("p", [190, 2500])
+def test_prefix_attention_graph(p):
     """A captured call sees the slot, the masks and the keys of each replay; two graphs and eager calls between them do not meet."""
-    b, g, h, hkv, p, t = 10, 2, 8, 2, 190, 50
+    b, g, h, hkv, t = 10, 2, 8, 2, 50
     args = inputs(b, g, 1, h, hkv, p, t, unused=0.5)
     gpu = [x.to(DEV) for x in args]
     slot, start = torch.zeros(1, dtype=I32, device=DEV), torch.zeros(g, dtype=I32, device=DEV)
