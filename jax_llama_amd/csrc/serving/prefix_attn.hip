@@ -22,6 +22,10 @@ constexpr int PA_TILE = PA_KT * PA_DH * 2;        // 16 KiB
 constexpr int PA_STEP = 32;                       // keys per step of a wave's 16 columns
 constexpr int PA_COLS = 128;
 
+// A step's 32 products in their order: 0 .. 15 of keys (two blocks of 32, 16 dims each), 16 + 4 ks + dt of values
+constexpr int PA_AHEAD = 3;  // operands are read from LDS this many products ahead (the first ones of keys: see the clearing of values)
+constexpr int PA_ORDER[32] = {0, 1, 2, 16, 3, 17, 4, 18, 5, 19, 6, 7, 8, 20, 9, 21, 10, 22, 11, 23, 12, 13, 24, 14, 25, 15, 26, 27, 28, 29, 30, 31};
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -34,6 +38,16 @@ JLA_DEV f32x16 mfma32(const u32x4 a, const u32x4 b, f32x16 c) {
 }
 JLA_DEV u32x2 ld_tr(const char* lds, int off) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + off)));
+}
+
+// LDS-DMA of 16 bytes a lane from base + off[j] to LDS bytes lds_wave + 4096 j .. + 1023 of a wave (kernels/common.h glds16_asm)
+JLA_DEV void glds16x4(const void* base, const int (&off)[4], unsigned lds_wave) {
+  asm volatile(
+      "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+      "s_add_i32 m0, m0, 4096\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %4\n\t"
+      "s_add_i32 m0, m0, 4096\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+      "s_add_i32 m0, m0, 4096\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %4" ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(lds_wave)
+      : "memory", "m0", "scc");
 }
 
 JLA_DEV int own_slot(const PrefixAttn& a) { return a.slot ? a.slot[0] : a.slot0; }
@@ -121,32 +135,42 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
     const int key = t.t0 + lane;
     return __ballot(key >= t.lo && key < t.hi && (!t.mask || t.mask[min(key, t.limit - 1)]));
   };
-  // else nothing of a tile is this wave's, nor of those after it
-  auto mine = [&](const Tile& t) { return active && (!t.own || t.t0 <= at_last); };
+  // A wave issues an instruction every 8 to 10 cycles, scalar ones too, and that bounds a step: what most tiles need is kept few. Tiles
+  // [plain, plain + n_plain) are the prefix's, whole and without a mask; from `past` on nothing is this wave's.
+  const int plain = pre.lo % PA_KT ? 1 : 0, n_plain = pre.mask ? 0 : max(0, n_pre - plain - (pre.hi % PA_KT ? 1 : 0));
+  auto is_plain = [&](int i) { return (unsigned)(i - plain) < (unsigned)n_plain; };
+  const int past = !active ? 0 : min(to, n_pre + max(0, ((at_last - own.first(PA_KT)) >> 6) + 1));
   auto slot_k = [&](int par) { return lds + par * PA_TILE; };
   auto slot_v = [&](int par) { return lds + (2 + par) * PA_TILE; };
+  const unsigned lds_w = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + 1024 * w;
   // 1-KiB blocks of 4 rows, lane L fills row L / 16, place L % 16 of its block (by asm: for the builtin the compiler waits before the
   // next read of LDS)
-  auto stage = [&](const bf16_t* src, const Tile& t, char* to_lds) {
+  int off[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int bi = w + 4 * j, row = 4 * bi + (lane >> 4);
-      const int ch = (lane & 15) ^ (((row & 3) << 2) | ((row >> 2) & 3));
-      glds16_asm(src + (size_t)t.t0 * PA_DH, 256 * min(row, t.limit - 1 - t.t0) + 16 * ch, to_lds + 1024 * bi);
+  for (int j = 0; j < 4; ++j) off[j] = 256 * (4 * (w + 4 * j) + (lane >> 4)) + 16 * ((lane & 15) ^ (((lane >> 4) << 2) | w));
+  auto stage = [&](const bf16_t* plain_at, const bf16_t* pre_at, const bf16_t* own_at, int i, int to_slot) {
+    if (is_plain(i)) {
+      glds16x4(plain_at + (size_t)i * (PA_KT * PA_DH), off, lds_w + to_slot * PA_TILE);
+    } else {
+      const Tile t = tile_of(i);
+      int at_row[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) at_row[j] = off[j] - 256 * max(0, 4 * (w + 4 * j) + (lane >> 4) - (t.limit - 1 - t.t0));
+      glds16x4((t.own ? own_at : pre_at) + (size_t)t.t0 * PA_DH, at_row, lds_w + to_slot * PA_TILE);
     }
   };
-  auto stage_k = [&](int i, int par) { const Tile t = tile_of(i); stage(t.k, t, slot_k(par)); };
-  auto stage_v = [&](int i, int par) { const Tile t = tile_of(i); stage(t.v, t, slot_v(par)); };
-
+  const size_t skipped = (size_t)pre.first(PA_KT) * PA_DH;
+  auto stage_k = [&](int i, int par) { stage(pre.k + skipped, pre.k, own.k, i, par); };
+  auto stage_v = [&](int i, int par) { stage(pre.v + skipped, pre.v, own.v, i, 2 + par); };
   // Tile i: K(i + 1) and V(i) are there, K(i + 2) and V(i + 1) on their way to the slots that tile i - 1 is done with. The scores of
   // tile i + 1 stand among the PV products of tile i, the exponentials of a key step among the products of the one before: the matrix
-  // unit (1024 cycles a tile and wave) and the vector unit (about 900) work side by side.
+  // unit (1024 cycles a tile and wave) and the vector unit (about 700) work side by side. 16 rows of 200 queries behind 4096 keys, us: the
+  // products in this order with their operands PA_AHEAD before them 246 (the compiler's, each operand read just before its product, 255),
+  // the maximum as one chain 234, the products before another wave's vector work 225.
   f32x16 sa[2], sb[2];
   const int k_off = pa_off(col, hi), v_off = pa_off(4 * (G >> 1) + gq, 2 * (G & 1) + (gp >> 1)) + 8 * (gp & 1);
-  auto score = [&](f32x16 (&s)[2], const char* kt, int f) {
-    const u32x4 k = *reinterpret_cast<const u32x4*>(kt + (k_off ^ (32 * (f >> 1))) + 8192 * (f & 1));
-    s[f & 1] = mfma32(k, qf[f >> 1], s[f & 1]);
-  };
+  auto key_frag = [&](const char* kt, int f) { return *reinterpret_cast<const u32x4*>(kt + (k_off ^ (32 * (f >> 1))) + 8192 * (f & 1)); };
+  auto score = [&](f32x16 (&s)[2], const u32x4 k, int f) { s[f & 1] = mfma32(k, qf[f >> 1], s[f & 1]); };
   auto clear = [&](f32x16 (&s)[2]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
@@ -171,8 +195,9 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
   };
   // what a tile needs before its PV: masks, the running maximum (it moves, and the sums with it, only where it grew by more than 8:
   // 2^(x - m) stays below 256), the weights of its first key step. raw: the largest score before masks
-  auto enter = [&](const Tile& t, uint64_t kept, f32x16 (&s)[2], float raw) {
-    if (kept != ~0ull || (t.own && t.t0 + PA_KT - 1 > at_first)) {
+  auto enter = [&](int i, uint64_t kept, f32x16 (&s)[2], float raw) {
+    const Tile t = tile_of(i);
+    if (!is_plain(i) && (kept != ~0ull || (t.own && t.t0 + PA_KT - 1 > at_first))) {
       uint64_t ok = kept;  // element e of block kb is key t0 + 4 hi + 32 kb + (e & 3) + 8 (e >> 2)
       const int n = at - t.t0 + 1;
       if (t.own && n < PA_KT) ok = n > 0 ? ok & ~(~0ull << n) : 0ull;
@@ -201,15 +226,21 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
     sum = 0.f;
     pf = weights(s, 0);
   };
-  auto pv = [&](const char* vt, int ks, int dt) {
+  auto value_frag = [&](const char* vt, int ks, int dt) {
     const u32x2 lo4 = ld_tr(vt, (v_off ^ (64 * dt)) + 4096 * ks), hi4 = ld_tr(vt, (v_off ^ (64 * dt) ^ 32) + 2048 + 4096 * ks);
-    o[dt] = mfma32(u32x4{lo4[0], lo4[1], hi4[0], hi4[1]}, pf, o[dt]);
+    return u32x4{lo4[0], lo4[1], hi4[0], hi4[1]};
   };
   uint64_t kept = ~0ull;  // tile i's
   auto step = [&](int i, auto parity, f32x16 (&s)[2], f32x16 (&next)[2]) {
     constexpr int par = decltype(parity)::value;
-    const Tile t = tile_of(i), tn = tile_of(min(i + 1, to - 1));
-    const uint64_t kept_next = kept_of(tn);
+    auto fetch = [&](int n) {
+      const int f = PA_ORDER[n];
+      return f < 16 ? key_frag(slot_k(par ^ 1), f) : value_frag(slot_v(par), (f - 16) >> 2, (f - 16) & 3);
+    };
+    u32x4 fr[PA_AHEAD + 1];
+#pragma unroll
+    for (int n = 0; n < PA_AHEAD; ++n) fr[n] = fetch(n);
+    const uint64_t kept_next = is_plain(i + 1) || i + 1 >= to ? ~0ull : kept_of(tile_of(i + 1));
     if (i + 2 < to) stage_k(i + 2, par);
     if (i + 1 < to) stage_v(i + 1, par ^ 1);
     if (kept != ~0ull) {  // values of keys that nobody attends may be anything: 0 x NaN would not be 0
@@ -220,40 +251,55 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
       }
       __syncthreads();
     }
-    if (mine(t)) {
+    if (i < past) {
+      __builtin_amdgcn_s_setprio(1);
       clear(next);
+      float e[8], most0 = -INFINITY, most1 = -INFINITY;
+      // (what an empty asm reads is computed before it: products and weights have no other order among themselves)
+      u32x4 after = pf;
 #pragma unroll
-      for (int ks = 0; ks < 3; ++ks) {
-        __builtin_amdgcn_sched_barrier(0);
+      for (int n = 0; n < 32; ++n) {
+        if (n + PA_AHEAD < 32) fr[(n + PA_AHEAD) % (PA_AHEAD + 1)] = fetch(n + PA_AHEAD);
+        // the weights of the next key step: an element a product, its sum one later, their packing before the step ends
+        const int ks = n < 20 ? n / 10 : n < 28 ? 2 : 3, q = n < 20 ? n % 10 : (n - 20) % 8;
+        if (ks < 3) {
+          const int first = ks == 2 ? (q ? q + 1 : 0) : q, count = ks == 2 ? (q == 0 ? 2 : q < 7 ? 1 : 0) : q < 8 ? 1 : 0;
 #pragma unroll
-        for (int f = 6 * ks; f < (ks < 2 ? 6 * ks + 6 : 16); ++f) score(next, slot_k(par ^ 1), f);
-        const u32x4 after = weights(s, ks + 1);
+          for (int j = first; j < first + count; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(fmaf(s[(ks + 1) >> 1][8 * ((ks + 1) & 1) + j], scale, -m_use));
+            asm volatile("" ::"v"(e[j]));
+            if (j) {
+              sum += e[j - 1];
+              asm volatile("" ::"v"(sum));
+            }
+          }
+          if (q == (ks == 2 ? 7 : 8)) {
+            sum += e[7];
+            after = pack8(e);
+          }
+        } else {  // the largest of the next tile's scores
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) pv(slot_v(par), ks, dt);
-        pf = after;
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int j = 0; j < (ks < 2 ? 10 : 8); ++j) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-          __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          for (int j = 4 * q; j < 4 * q + 4; j += 2) {
+            most0 = fmaxf(fmaxf(most0, next[0][j]), next[0][j + 1]);
+            most1 = fmaxf(fmaxf(most1, next[1][j]), next[1][j + 1]);
+          }
         }
+        const int f = PA_ORDER[n];
+        if (f < 16) {
+          score(next, fr[n % (PA_AHEAD + 1)], f);
+          asm volatile("" ::"v"(next[f & 1]));
+        } else {
+          o[f & 3] = mfma32(fr[n % (PA_AHEAD + 1)], pf, o[f & 3]);
+          asm volatile("" ::"v"(o[f & 3]));
+        }
+        if (n == 9 || n == 19 || n == 27) pf = after;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(0);
       l_run += sum;  // (this half's keys; the halves meet at the end)
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) pv(slot_v(par), 3, dt);
-      const float raw = largest(next);
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (i + 1 < to && mine(tn)) enter(tn, kept_next, next, raw);
+      float raw = fmaxf(most0, most1);
+      asm volatile("" ::"v"(raw));
+      if (i + 1 < past) enter(i + 1, kept_next, next, raw);
     }
     kept = kept_next;
     wait_vmcnt<0>();
@@ -265,15 +311,14 @@ JLA_DEV void column_tile(const PrefixAttn& a, const PrefixPlan& p, int part, int
     if (from + 1 < to) stage_k(from + 1, 1);
     wait_vmcnt<0>();
     __syncthreads();
-    const Tile t = tile_of(from);
-    if (mine(t)) {
+    if (from < past) {
       clear(sa);
 #pragma unroll
-      for (int f = 0; f < 16; ++f) score(sa, slot_k(0), f);
+      for (int f = 0; f < 16; ++f) score(sa, key_frag(slot_k(0), f), f);
     }
     if (from + 2 < to) __syncthreads();  // K(from + 2) goes where K(from) was
-    kept = kept_of(t);
-    if (mine(t)) enter(t, kept, sa, largest(sa));
+    kept = kept_of(tile_of(from));
+    if (from < past) enter(from, kept, sa, largest(sa));
     for (int i = from; i < to; i += 2) {
       step(i, std::integral_constant<int, 0>{}, sa, sb);
       if (i + 1 < to) step(i + 1, std::integral_constant<int, 1>{}, sb, sa);
@@ -488,13 +533,14 @@ __global__ void __launch_bounds__(256, 2) prefix_attn_kernel(PrefixAttn a, Prefi
   __shared__ __attribute__((aligned(16))) char lds[4 * PA_TILE];
   const int rep = a.rep, n = a.n;
   if ((int)blockIdx.x < tiles) {
-    // (kv heads first: where they are a multiple of the 8 XCDs, all tiles that read the same keys run on one of them, behind one L2)
+    // Kv heads first, then columns: where kv heads are a multiple of the 8 XCDs, all tiles that read the same keys run on one of them,
+    // behind one L2, and at the same time (64 rows behind 65536 keys, two tiles of columns: 91 us, 101 with the keys' parts first).
     int id = blockIdx.x;
     const int kvh = id % a.Hkv;
     id /= a.Hkv;
-    const int part = id % p.ns;
-    id /= p.ns;
-    const int ct = id % p.ct, u = id / p.ct;
+    const int ct = id % p.ct;
+    id /= p.ct;
+    const int part = id % p.ns, u = id / p.ns;
     const int ncols = (p.by_row ? 1 : n) * a.S * rep;
     KeyRange own = own_keys(a, u, kvh, (min(ncols, (ct + 1) * PA_COLS) - 1) / rep);  // (by a group's number: row u exists too)
     if (!p.by_row) own.hi = own.lo;
@@ -552,42 +598,51 @@ static int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Which queries share a workgroup, and how the keys are split.
 //
-// A row's own columns go over prefix and own keys together from 96 of them on, else a group's over the prefix with the own keys beside:
-// 16 rows behind 4096 tokens, 8 kv heads, us shared | by row: 16 columns each 30 | 31, 64 41 | 46, 96 59 | 53, 224 106 | 94.
-//
-// Splits: a tile takes 1.15 us where a compute unit has one workgroup and 2.05 where it has two, in rounds of 512; each part's sums are
-// written and read at about 4.5 TB/s, and their join costs a launch. The fewest splits of the least time that makes: 32 rows behind 2048
-// tokens 16.5 us with 12 splits (4: 20.9, 32: 19.1), 200 behind 16384 73.8 with 9 (4: 97), 1000 queries of one row behind 8000 171 with 2
-// (1: 186, 3: 181), 200 queries of 4 rows behind 2000 51 with 1 (2: 65).
-PrefixPlan prefix_attn_plan(int B, int S, int H, int Hkv, int G, int P, int T) {
+// A row's own columns go over prefix and own keys together (by_row), or a group's over the prefix with the own keys beside; each with the
+// fewest splits of the least time by this model, in us: a tile takes 1.05 where a compute unit has one workgroup and 1.65 where it has two,
+// in rounds of 512; a wave's step of own keys 1.2 beside those, and 0.6 with 2048 under way; each part's sums are written and read at about 4.5 TB/s, and their
+// join costs a launch. Measured, by splits: 32 rows behind 2048 tokens 16.0 with 8 and 12 (4: 18.3, 32: 18.7), 200 behind 16384 72 with 9
+// (4: 79, 12: 88), 1000 queries of one row behind 8000 152 with 1 (2: 161, 3: 185). Shared | by row, 16 rows behind 4096 tokens: 16 columns
+// each 21.7 | 39, 64 36.7 | 48, 144 62.8 | 71.6, 192 80 | 70; 64 rows of 100 columns behind 1000 79 | 40.5; a row alone is by
+// row (behind 32768 tokens with 2000 of its own 36 | 29, 8 of them behind 8192 45.7 | 44.8).
+static PrefixPlan plan_of(int B, int S, int H, int Hkv, int G, int P, int T, bool by_row, double& best) {
   PrefixPlan p{};
   const int rep = H / Hkv, n = B / G;
-  p.by_row = S * rep >= 96;
-  const int cols = (p.by_row ? 1 : n) * S * rep, keys = ceil_div(P, PA_KT) + (p.by_row ? ceil_div(T, PA_KT) : 0);
-  p.ct = ceil_div(cols, PA_COLS);
-  const long long tiles = (long long)(p.by_row ? B : G) * Hkv * p.ct;
+  p.by_row = by_row;
+  const long long cols = (long long)(by_row ? 1 : n) * S * rep;
+  const int keys = ceil_div(P, PA_KT) + (by_row ? ceil_div(T, PA_KT) : 0);
+  p.ct = (int)((cols + PA_COLS - 1) / PA_COLS);
+  const long long tiles = (long long)(by_row ? B : G) * Hkv * p.ct;
+  const double part = 2. * 4 * (PA_DH + 2) * B * S * H / 4.5e6;
   auto tiles_time = [&](int ns) {
     const long long groups = tiles * ns, rest = groups % 512;
-    return ceil_div(keys, ns) * ((double)(groups / 512) * 2.05 + (rest == 0 ? 0. : rest <= 256 ? 1.15 : 2.05));
+    return ceil_div(keys, ns) * ((double)(groups / 512) * 1.65 + (rest == 0 ? 0. : rest <= 256 ? 1.05 : 1.65));
   };
-  const double part = 2. * 4 * (PA_DH + 2) * B * S * H / 4.5e6;  // us
-  double best = 1e30;
-  p.ns = 1;
-  for (int ns = 1; ns <= keys && ns <= 256; ++ns) {
-    const double t = tiles_time(ns) + (p.by_row && ns == 1 ? 0. : part * ns + 3.5);
+  best = 1e30;
+  for (int ns = 1; ns <= keys && (ns == 1 || tiles * ns <= 1024); ++ns) {
+    const double t = tiles_time(ns) + (by_row && ns == 1 ? 0. : part * ns + 3.5);
     if (t < best) best = t, p.ns = ns;
   }
-  if (!p.by_row) {  // own keys: a wave's step takes about 0.6 us; as long as the prefix's tiles run, or 3
+  if (!by_row) {  // own keys as long as the prefix's tiles run, or 3 us
     p.own_ct = ceil_div(S * rep, 16);
-    const double steps = ceil_div(T, PA_STEP) * 0.6, beside = tiles_time(p.ns) > 3. ? tiles_time(p.ns) : 3.;
+    const double steps = ceil_div(T, PA_STEP), beside = tiles_time(p.ns) > 3. ? tiles_time(p.ns) : 3.;
     const long long waves = (long long)B * Hkv * p.own_ct, most = waves >= 2048 ? 1 : 2048 / waves;
-    const long long want = (long long)(steps / beside) + 1;
+    const long long want = (long long)(1.2 * steps / beside) + 1;
     p.own_ns = (int)(want < most ? want : most);
+    best += part * p.own_ns + 0.6 * steps * waves / 2048;
   }
+  return p;
+}
+
+PrefixPlan prefix_attn_plan(int B, int S, int H, int Hkv, int G, int P, int T) {
+  double best, by_row;
+  PrefixPlan p = plan_of(B, S, H, Hkv, G, P, T, false, best);
+  const PrefixPlan rows = plan_of(B, S, H, Hkv, G, P, T, true, by_row);
+  if (B == G || by_row < best) p = rows, best = by_row;
   // Short ones in one launch, 16 columns a workgroup: a step of its eight waves takes about 2 us (128 KiB through one compute unit), against 0.9
   // us more for the two launches: 2 rows behind 130 tokens 5.5 us (8.3), 32 behind 250 7.5 (11.8), 8 behind 700 11.4 (9.8), 64 behind 250
   // 13.0 (12.9).
-  const int rows_ct = ceil_div(S * rep, 16), steps = ceil_div(ceil_div(P, PA_STEP) + ceil_div(T, PA_STEP), PS_WAVES);
+  const int rows_ct = ceil_div(S * (H / Hkv), 16), steps = ceil_div(ceil_div(P, PA_STEP) + ceil_div(T, PA_STEP), PS_WAVES);
   const double rounds = (double)(((long long)B * Hkv * rows_ct + 255) / 256);
   if (rounds * steps * (rounds > 1. ? 2.4 : 2.) < best + 0.9) p.brief = 1, p.own_ct = rows_ct;
   return p;
