@@ -168,7 +168,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     outside the columns are passed over. A penalty is a number or fp32 ``[B]``. ``allowed``: int32 bits ``[masks, words]``
     (``pack_allowed``), one mask for all, one per row, or row ``allowed_rows[b]`` of them (int32 ``[B]``; an index outside the masks allows
     everything). ``vocab_start``: token id of column 0 (a vocabulary shard); ``bias`` has the shard's columns, ``allowed`` all ids.
-    ``out``: ``logits`` itself (in place; without bias and mask only the history's tokens are touched) or another tensor."""
+    ``out``: ``logits`` itself (in place) or another tensor."""
     if logits.device.type == "cuda":
         return ext().process_logits(logits, out, history, length, start, history_mask, prompt_len, vocab_start, repetition_penalty,
                                     presence_penalty, frequency_penalty, bias, allowed, allowed_rows)

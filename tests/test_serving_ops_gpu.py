@@ -193,7 +193,8 @@ def packed(kw):
     return dev({**kw, "allowed": ops.pack_allowed(kw["allowed"]) if kw.get("allowed") is not None else None})
 
 
-@pytest.mark.parametrize("b,v,n", [(1, 1, 1), (1, 2, 0), (3, 33, 9), (2, 8191, 300), (2, 8192, 40), (3, 8193, 700), (2, 32001, 2500), (5, 128256, 90)])
+@pytest.mark.parametrize("b,v,n", [(1, 1, 1), (1, 2, 0), (3, 33, 9), (2, 8191, 300), (2, 8192, 40), (3, 8193, 700), (2, 32001, 2500), (5, 128256, 90), (17, 128256, 50),
+                                   (150, 14001, 600)])
 def test_process_logits(b, v, n):
     x, kw = torch.randn(b, v) * 3, logits_inputs(b, v, n, 4)
     for drop in ((), ("bias",), ("allowed", "allowed_rows"), ("bias", "allowed", "allowed_rows"), ("start", "history_mask"),
