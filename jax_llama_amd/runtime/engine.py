@@ -273,13 +273,13 @@ class DecodeEngine:
             held = 0
         else:
             self.kv_start.copy_(each(start))
-            self.key_mask = key_mask
+            self.key_mask = each(key_mask) if key_mask is not None else None
             if n == 1:
                 logits = self._prefill_rows(ids, pos_dev, self.cache, self.kv_start, key_mask)
             else:
                 own = self.cache.own if self.prefix is not None else self.cache
                 rows = own.rows(0, b)
-                logits = self._prefill_rows(ids, pos_dev, SharedPrefixCache(self.prefix, rows) if self.prefix is not None else rows, start, None)
+                logits = self._prefill_rows(ids, pos_dev, SharedPrefixCache(self.prefix, rows) if self.prefix is not None else rows, start, key_mask)
                 own.copy_rows([i // n for i in range(self.b)], range(self.b), tokens=s)
         self.cache.advance(held)
         # state for the loop body: cur_len = S (also the sampler's Philox step), token/pos of the

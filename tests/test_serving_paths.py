@@ -237,6 +237,16 @@ def test_samples_of_layer_list_models(device, name):
         model.generate(ids, None, gc, prefix=KVCache(1, 1, 1, 4, 16, "cpu"))
 
 
+@pytest.mark.parametrize("name", ["besulix", "zavevik"])
+def test_samples_of_layer_list_models_refuse_holes(name):
+    """As one sample of a prompt with holes in its mask does."""
+    model, ids, mask = family(name, "cpu"), torch.randint(3, 37, (2, 9), dtype=torch.int32), torch.ones(2, 9, dtype=torch.int32)
+    mask[1, 4] = 0
+    for n in (1, 3):
+        with pytest.raises(NotImplementedError):
+            model.generate(ids, mask, config(4, 9, do_sample=True), num_return_sequences=n)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("name", ["besulix", "zavevik"])
 def test_forked_requests(device, name):
