@@ -346,7 +346,11 @@ class LLaMAForCausalLM:
                 raise ValueError("a prefix may be padded on the left only")
             cache.start = start
             pos = (mask.cumsum(-1) - 1).to(torch.int32).to(self.device)
-        self.forward_tokens(ids, pos, cache, 0, start, logits_mode="none")
+        from ..runtime.engine import PREFILL_TOKENS
+        rows = max(1, PREFILL_TOKENS // max(1, p))
+        for b0 in range(0, g, rows):
+            part = slice(b0, min(g, b0 + rows))
+            self.forward_tokens(ids[part], pos[part], cache.rows(part.start, part.stop) if rows < g else cache, 0, start[part], logits_mode="none")
         cache.advance(p)
         return cache
 

@@ -342,7 +342,8 @@ class DecodeEngine:
         return (c.prefix.k.data_ptr(), c.prefix.v.data_ptr(), *(t.data_ptr() if t is not None else 0 for t in (c.start, c.mask)))
 
     def nbytes(self) -> int:
-        return self.cache.nbytes() + (self.prompt_cache.nbytes() if self.prompt_cache is not None else 0)
+        """Of the caches it keeps alive (a prefix counts in each engine behind it)."""
+        return sum(c.nbytes() for c in (self.cache, self.prompt_cache, self.prefix) if c is not None)
 
     def _ensure_graph(self):
         if self._graph is not None and self._graph_key == self._graph_state():
@@ -454,6 +455,8 @@ def get_engine(model, batch_size: int, max_length: int, samples: int = 1, prompt
     else:
         tokens = batch_size * prompt_len + rows * (max_length - prompt_len) if shared else rows * max_length
         need = model.config.num_hidden_layers * 2 * tokens * model.n_kv_heads * model.head_dim * 2
+    if prefix is not None:
+        need += prefix.nbytes()
     budget = _engine_budget(model)
     held = sum(e.nbytes() for e in _ENGINES.values())
     while _ENGINES and held + need > budget:

@@ -205,6 +205,23 @@ class _Tokenizer:
         return " ".join(map(str, ids))
 
 
+def test_prefixes_in_chunks_and_the_bytes_of_engines(monkeypatch):
+    """Many prefixes run through the model some rows at a time; a prefix that an engine keeps alive counts towards the engines' bytes."""
+    model, head, ids = llama("cpu"), prompts(5, 13), prompts(5, 4, seed=6)
+    whole = model.encode_prefix(head, left_padded(5, 13))
+    monkeypatch.setattr(engine, "PREFILL_TOKENS", 30)  # 2 rows, 2, 1
+    cut = model.encode_prefix(head, left_padded(5, 13))
+    assert torch.equal(whole.k, cut.k) and torch.equal(whole.v, cut.v) and torch.equal(whole.start, cut.start) and cut.index == 13
+    model.generate(ids, None, config(3, 4), prefix=cut)
+    eng, = engine._ENGINES.values()
+    assert eng.nbytes() == eng.cache.own.nbytes() + cut.nbytes()
+    monkeypatch.setattr(engine, "_engine_budget", lambda m: 3 * eng.nbytes())
+    kept = [model.encode_prefix(head) for _ in range(6)]
+    for prefix in kept:
+        model.generate(ids, None, config(3, 4), prefix=prefix)
+    assert [e.prefix for e in engine._ENGINES.values()] == kept[3:]
+
+
 def test_generator_strings():
     gen = LLaMA(None, llama("cpu"), _Tokenizer())
     out = gen.generate_from_str(["ab", "cde"], 5, num_return_sequences=2, repetition_penalty=1.2)
