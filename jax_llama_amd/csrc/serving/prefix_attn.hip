@@ -9,6 +9,7 @@
 // Columns. The queries of one kv head that read the same keys are the columns of S^T = K Q^T: for a prefix n S rep of them (n rows of
 // its group, rep query heads per kv head, column c = token (c / rep), head (c % rep)), for a row's own keys S rep. So a prefix is
 // read once per 128 columns instead of once per row.
+#include <atomic>
 #include <type_traits>
 
 #include "../kernels/common.h"
@@ -656,8 +657,15 @@ int prefix_attn(const PrefixAttn& a, const PrefixPlan& p, hipStream_t s) {
   if (a.B <= 0 || a.S <= 0) return 0;
   if (a.H % a.Hkv || a.G <= 0 || a.B % a.G || a.P < 1 || a.T < 1) return -1;
   if (p.brief) {
-    static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_short_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PS_LDS);
-    if (room != hipSuccess) return (int)room;
+    static std::atomic<unsigned long long> has_room{0};  // a bit for each of the first devices: the limit is a device's
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return (int)e;
+    if (device >= 64 || !(has_room.load() >> device & 1)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_short_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PS_LDS);
+      if (e != hipSuccess) return (int)e;
+      if (device < 64) has_room |= 1ull << device;
+    }
     const long long items = (long long)a.B * a.Hkv * p.own_ct;
     if (items > 0x7fffffff) return -3;
     prefix_short_kernel<<<(int)items, 64 * PS_WAVES, PS_LDS, s>>>(a, p);

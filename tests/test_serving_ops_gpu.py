@@ -132,6 +132,52 @@ def test_prefix_attention_views_streams_and_packed(p):
     assert torch.equal(rows, got.view(torch.int16))
 
 
+@pytest.mark.parametrize("p", [100, 2500])
+def test_prefix_attention_rows_past_32_bits(p):
+    """The second prefix lies 2^31 elements behind the first."""
+    q, kp, vp, ko, vo = inputs(6, 2, 1, 8, 2, p, 30, slot=20)
+    want, bound = oracle.prefix_attention(q, kp, vp, ko, vo, 20)
+    n = 2 * p * 128
+    far = torch.empty(2 ** 31 + 2 * n, dtype=BF16, device=DEV)
+    views = [far.as_strided((2, 2, p, 128), (2 ** 31, p * 128, 128, 1), at) for at in (0, n)]
+    for view, x in zip(views, (kp, vp)):
+        view.copy_(x)
+    close(ops.prefix_attention(q.to(DEV), *views, ko.to(DEV), vo.to(DEV), 20), want, bound)
+
+
+@pytest.mark.parametrize("s,h", [(1, 2), (60, 2)])
+def test_prefix_attention_tokens_past_32_bits(s, h):
+    """The last keys of a prefix of 2^24 tokens (2^31 elements) and of own keys as far in; the others are unset and not attended."""
+    far, live = 2 ** 24 + 77, 500
+    q, kp, vp, ko, vo = inputs(2, 1, s, h, 1, live, live, slot=live - s)
+    want, bound = oracle.prefix_attention(q, kp, vp, ko, vo, live - s)
+    k, v = (torch.empty(2, 1, far, 128, dtype=BF16, device=DEV) for _ in range(2))
+    for x, a, b in ((k, kp, ko), (v, vp, vo)):
+        x[:1, :, far - live:] = a.to(DEV)
+    start = torch.full((1,), far - live, dtype=I32, device=DEV)
+    close(ops.prefix_attention(q.to(DEV), k[:1], v[:1], ko.to(DEV), vo.to(DEV), live - s, prefix_start=start), want, bound)
+    for x, b in ((k, ko), (v, vo)):
+        x[:, :, far - live:] = b.to(DEV)
+    close(ops.prefix_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, far - s, kv_start=start.expand(2).contiguous()), want, bound)
+
+
+@pytest.mark.parametrize("p", [100, 2500])
+def test_prefix_attention_two_streams(p):
+    """Calls under way at once on two streams have parts of their own."""
+    sets = [[x.to(DEV) for x in inputs(12, 2, 1, 8, 2, p, 30, slot=20)] for _ in range(2)]
+    want = [ops.prefix_attention(*s, 20) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.prefix_attention(*sets[i], 20))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
 @pytest.mark.parametrize("p", [190, 2500])
 def test_prefix_attention_graph(p):
     """A captured call sees the slot, the masks and the keys of each replay; two graphs and eager calls between them do not meet."""
@@ -226,6 +272,23 @@ def test_process_logits_strides_rows_and_shards():
     for cut in (1, 31, 32, 500, 1000):
         parts = [ops.process_logits(x[:, a:z].to(DEV), vocab_start=a, **{**packed(kw), "bias": kw["bias"][:, a:z].to(DEV)}) for a, z in ((0, cut), (cut, v))]
         assert torch.equal(torch.cat(parts, 1), want)
+
+
+def test_process_logits_past_32_bits():
+    """Rows behind 2^31 elements, out of place and in place."""
+    v = 32000
+    b = 2 ** 31 // v + 5
+    x = torch.empty(b, v, device=DEV)
+    x[-4:] = torch.randn(4, v)
+    kw = packed({k: t for k, t in logits_inputs(b, v, 40, 3).items() if k != "bias"})
+    last = {k: t[-4:].contiguous() if torch.is_tensor(t) and t.shape[0] == b else t for k, t in kw.items()}
+    want = ops.process_logits(x[-4:].clone(), **last)
+    assert torch.equal(ops.process_logits(x, **kw)[-4:], want)
+    for k in ("allowed", "allowed_rows"):
+        kw.pop(k), last.pop(k)
+    want = ops.process_logits(x[-4:].clone(), **last)
+    ops.process_logits(x, out=x, **kw)
+    assert torch.equal(x[-4:], want)
 
 
 def test_process_logits_masked_nan_and_dead_ends():
