@@ -17,40 +17,45 @@ class RowLayout:
 
     def __init__(self, rows: int, layers: Sequence[torch.Tensor] = (), tokens: Sequence[torch.Tensor] = (), state: Sequence[torch.Tensor] = ()):
         self.rows = rows
-        self.tensors: List[Tuple[torch.Tensor, bool]] = []  # (a layer's, whether it has tokens)
+        self.layers, self.tensors = list(layers), [(t, True) for t in tokens] + [(t, False) for t in state if t.numel()]
         self.parts: List[Tuple[int, ...]] = []
         self.types: List[torch.dtype] = []
         self.words: List[int] = []  # eight numbers a span: csrc/serving/serving.h RowSpan
-        for t in layers:
-            self._add(t[0], True, t.shape[0], t.stride(0))
-            self.tensors += [(x, True) for x in t]
-        for t, has in [(t, True) for t in tokens] + [(t, False) for t in state if t.numel()]:
-            self._add(t, has, 1, 0)
-            self.tensors.append((t, has))
+        for t in self.layers:
+            self._add(t, t.shape[1:], t.stride()[1:], True, t.shape[0], t.stride(0))
+        for t, has in self.tensors:
+            self._add(t, t.shape, t.stride(), has, 1, 0)
+        held = self.layers + [t for t, _ in self.tensors]
+        self.on = held[0] if held and held[0].device.type == "cuda" else None
         self._native = None
 
-    def _add(self, t: torch.Tensor, has_tokens: bool, layers: int, layer_stride: int) -> None:
+    def _add(self, t: torch.Tensor, shape, stride, has_tokens: bool, layers: int, layer_stride: int) -> None:
         es = t.element_size()
         if has_tokens:
-            ok, part = t.stride(3) == 1 and t.stride(2) == t.shape[3], (layers, t.shape[1], t.shape[3] * es, 0)
+            ok, part = stride[3] == 1 and stride[2] == shape[3], (layers, shape[1], shape[3] * es, 0)
         else:
-            ok, part = t[0].is_contiguous(), (layers, 1, 0, t[0].numel() * es)
+            ok, n = True, 1
+            for size, step in zip(reversed(shape[1:]), reversed(stride[1:])):
+                ok, n = ok and (size == 1 or step == n), n * size
+            part = (layers, 1, 0, n * es)
         if not ok:
             raise ValueError("a cache row must be one piece of each of its tensors")
         self.types.append(t.dtype)
-        self.words += [t.data_ptr(), t.stride(0) * es, layer_stride * es, t.stride(1) * es if has_tokens else 0, *part]
+        self.words += [t.data_ptr(), stride[0] * es, layer_stride * es, stride[1] * es if has_tokens else 0, *part]
         self.parts.append(part)
 
     def copy(self, to: "RowLayout", src: Sequence[int], dst: Sequence[int], tokens: int) -> None:
         """Row ``dst[i]`` of ``to`` becomes row ``src[i]`` (``NOTHING``: zeros). ``to is self``: every source is read as it was before."""
         if self.types != to.types:
             raise ValueError("the caches are laid out differently")
-        if not self.tensors or self.tensors[0][0].device.type != "cuda":
+        if (self.on is None) != (to.on is None):
+            raise ValueError("the caches lie on different devices")
+        if self.on is None:
             self._copy_cpu(to, [int(r) for r in src], [int(r) for r in dst], tokens)
             return
         for a in (self, to):
             if a._native is None:
-                a._native = serving.ext().RowLayout(a.words, a.rows, a.tensors[0][0])
+                a._native = serving.ext().RowLayout(a.words, a.rows, a.on)
         self._native.copy(to._native, src, dst, tokens)
 
     def _copy_cpu(self, to: "RowLayout", src: List[int], dst: List[int], tokens: int) -> None:
@@ -64,7 +69,9 @@ class RowLayout:
             raise ValueError(f"rows {dst} of a cache of {to.rows}")
         if len(set(dst)) != len(dst):
             raise ValueError(f"a row is written twice: {dst}")
-        for (t, has), (o, _) in zip(self.tensors, to.tensors):
+        def each(a):
+            return [(x, True) for t in a.layers for x in t] + a.tensors
+        for (t, has), (o, _) in zip(each(self), each(to)):
             def part(x, row):
                 return x[row, :, :tokens] if has else x[row]
             held = [torch.zeros_like(part(o, d)) if s == NOTHING else part(t, s).clone() for s, d in zip(src, dst)]

@@ -391,6 +391,10 @@ def test_copy_rows_refusals_gpu():
                              ([0], [1], dict(tokens=7)), ([0], [1], dict(tokens=-1))):
             with pytest.raises(ValueError):
                 cache.copy_rows(src, dst, **kw)
+    cpu = KVCache(2, 4, 2, 6, 128, "cpu")
+    for a, b in ((kv, cpu), (cpu, kv)):
+        with pytest.raises(ValueError):
+            a.copy_rows([0], [1], tokens=1, to=b)
     for other in (hy, KVCache(2, 4, 3, 6, 128, DEV), KVCache(3, 4, 2, 6, 128, DEV), KVCache(2, 4, 2, 6, 64, DEV, torch.float32)):
         with pytest.raises(ValueError):
             kv.copy_rows([0], [1], tokens=1, to=other)
