@@ -339,6 +339,7 @@ struct RowLayout {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefix_attn", &prefix_attn, py::arg("q"), py::arg("kp"), py::arg("vp"), py::arg("ko"), py::arg("vo"), py::arg("slot"),
         py::arg("prefix_len"), py::arg("prefix_start"), py::arg("prefix_mask"), py::arg("kv_start"), py::arg("out_pack"));
+  // the way a call of these sizes goes: in one launch, by row or by group, with a join or without
   m.def("prefix_plan", [](int b, int s, int h, int hkv, int g, int p, int t) {
     const jla::PrefixPlan plan = jla::prefix_attn_plan(b, s, h, hkv, g, p, t);
     return std::string(plan.brief ? "short" : plan.by_row ? "row" : "group") + (!plan.brief && plan.parts() > 1 ? "+join" : "");
