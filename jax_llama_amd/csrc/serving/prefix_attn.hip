@@ -642,12 +642,13 @@ PrefixPlan prefix_attn_plan(int B, int S, int H, int Hkv, int G, int P, int T) {
   PrefixPlan p = plan_of(B, S, H, Hkv, G, P, T, false, best);
   const PrefixPlan rows = plan_of(B, S, H, Hkv, G, P, T, true, by_row);
   if (B == G || by_row < best) p = rows, best = by_row;
-  // Short ones in one launch, 16 columns a workgroup: a step of its eight waves takes about 2 us (128 KiB through one compute unit), against 0.9
-  // us more for the two launches: 2 rows behind 130 tokens 5.5 us (8.3), 32 behind 250 7.5 (11.8), 8 behind 700 11.4 (9.8), 64 behind 250
-  // 13.0 (12.9).
+  // Short ones in one launch, 16 columns a workgroup: a step of its eight waves takes about 2 us (128 KiB through one compute unit), less in
+  // several rounds; the two launches take some 0.6 us more than the sum above. One | two launches, us: 2 rows behind 130 tokens 5.5 | 9.3, 32
+  // behind 250 7.2 | 10.5, 32 behind 700 10.5 | 13.4, 8 of 8 queries behind 300 7.9 | 11.0, 8 behind 700 10.3 | 9.6, 4 behind 1000 13.3 | 9.5, 128 behind
+  // 130 18.1 | 16.0, 8 of 64 queries behind 200 24.6 | 12.8.
   const int rows_ct = ceil_div(S * (H / Hkv), 16), steps = ceil_div(ceil_div(P, PA_STEP) + ceil_div(T, PA_STEP), PS_WAVES);
-  const double rounds = (double)(((long long)B * Hkv * rows_ct + 255) / 256);
-  if (rounds * steps * (rounds > 1. ? 2.4 : 2.) < best + 0.9) p.brief = 1, p.own_ct = rows_ct;
+  const long long rounds = ((long long)B * Hkv * rows_ct + 255) / 256;
+  if ((rounds == 1 ? 2. * steps : 1.5 * rounds * (steps + 1)) < best + 0.6) p.brief = 1, p.own_ct = rows_ct;
   return p;
 }
 

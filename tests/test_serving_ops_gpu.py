@@ -45,7 +45,8 @@ SHAPES = [  # and the way they go (csrc/serving/prefix_attn.hip prefix_attn_plan
     (4, 2, 2, 6, 2, 2200, 130, 100, "group+join"),  # two queries a row
     (9, 3, 1, 6, 2, 1025, 300, 290, "group+join"),
     (2, 1, 1, 4, 1, 4100, 1200, 1111, "row+join"), 
-    (70, 7, 3, 20, 4, 700, 40, 8, "group+join"),    # 5 query heads, 150 columns a prefix, 15 of own keys
+    (70, 7, 3, 20, 4, 700, 40, 8, "short"),         # 5 query heads, 280 workgroups
+    (70, 7, 3, 20, 4, 1100, 40, 8, "group+join"),   # 150 columns a prefix, 15 of own keys
     (3, 1, 130, 4, 2, 1257, 200, 66, "row+join"),   # tiles of one row over both
     (1, 1, 96, 1, 1, 1000, 96, 0, "row+join"),
     (64, 2, 60, 8, 4, 500, 80, 20, "row"),          # 120 columns a row, one part
