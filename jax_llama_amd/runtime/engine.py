@@ -132,7 +132,7 @@ def _sample(model, logits_local: torch.Tensor, gc: GenerationConfig, gen: Option
         keep[:, 0] = True
         vals = torch.where(keep, vals, torch.full_like(vals, _NEG_INF))
     u = torch.rand(vals.shape, device=vals.device, generator=gen, dtype=torch.float32)
-    gumbel = -torch.log(-torch.log(u.clamp_min(1e-20)).clamp_min(1e-20))
+    gumbel = -torch.log((-torch.log(u.clamp_min(1e-20))).clamp_min(1e-20))
     choice = (vals + gumbel).argmax(-1)
     return idx.gather(1, choice[:, None]).squeeze(1).to(torch.int32)
 
