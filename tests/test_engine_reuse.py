@@ -1,0 +1,69 @@
+"""One engine over calls that differ: what a captured step has baked in is that of the present call. CPU here, the captured steps with -m gpu."""
+import pytest
+import torch
+
+from jax_llama_amd import GenerationConfig, LLaMAConfig, LLaMAForCausalLM
+from jax_llama_amd.runtime.engine import DecodeEngine
+
+DEVICES = ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)]
+V = 96
+
+
+def model_of(device):
+    cfg = LLaMAConfig(vocab_size=V, hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+                      num_key_value_heads=1, max_sequence_length=128, rms_norm_eps=1e-5)
+    return LLaMAForCausalLM(cfg, device=device, _do_init=False).init_random(seed=3, std=0.12)
+
+
+def prompts(b, s, seed=0):
+    return torch.randint(3, V, (b, s), generator=torch.Generator().manual_seed(seed), dtype=torch.int32)
+
+
+def config(**kw):
+    return GenerationConfig(**{**dict(max_length=26, do_sample=True, temperature=1.5, top_k=20, top_p=0.95, seed=1, pad_token_id=0, eos_token_id=-1), **kw})
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sampling_settings_of_the_present_call(device):
+    model, ids = model_of(device), prompts(3, 8)
+    kept = DecodeEngine(model, 3, 26)
+    seen = []
+    for kw in (dict(), dict(seed=2), dict(temperature=0.8), dict(top_p=0.7), dict(top_k=5), dict(top_k=0), dict(top_k=0, temperature=0.9), dict(),
+               dict(seed=2 ** 40 + 1), dict(do_sample=False), dict(do_sample=False, seed=7)):
+        got = kept.run(ids, None, config(**kw)).cpu().clone()
+        assert torch.equal(got, DecodeEngine(model, 3, 26).run(ids, None, config(**kw)).cpu()), kw
+        seen.append(tuple(got.reshape(-1).tolist()))
+    assert len(set(seen)) == 9  # (the first twice, greedy twice)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("sampled", [False, True])
+def test_end_and_pad_tokens_of_the_present_call(device, sampled):
+    model, ids = model_of(device), prompts(3, 8)
+    kept = DecodeEngine(model, 3, 26)
+    free = kept.run(ids, None, config(do_sample=sampled)).cpu().clone()
+    for at, pad in ((14, 0), (17, 1), (14, 2)):  # the end tokens: what the first row says late
+        gc = config(do_sample=sampled, eos_token_id=int(free[0, at]), pad_token_id=pad)
+        got = kept.run(ids, None, gc).cpu().clone()
+        first = free[0].tolist().index(gc.eos_token_id, 8)
+        assert got[0].tolist() == free[0, :first + 1].tolist() + [pad] * (25 - first)
+        assert torch.equal(got, DecodeEngine(model, 3, 26).run(ids, None, gc).cpu())
+
+
+def test_state_of_a_captured_step():
+    """A greedy step does not depend on what is for sampling: it is not captured again."""
+    model = model_of("cpu")
+    eng = DecodeEngine(model, 2, 20)
+    ids = prompts(2, 8)
+
+    def state(**kw):
+        eng.prefill_only(ids, None, config(max_length=20, **kw))
+        return eng._graph_state()
+
+    base = state()
+    for kw in (dict(seed=2), dict(temperature=0.5), dict(top_p=0.5), dict(top_k=4), dict(eos_token_id=5), dict(pad_token_id=3), dict(do_sample=False)):
+        assert state(**kw) != base
+    assert state() == base
+    greedy = state(do_sample=False)
+    assert state(do_sample=False, seed=9, temperature=0.1, top_k=1, top_p=0.2) == greedy
+    assert state(do_sample=False, eos_token_id=4) != greedy
