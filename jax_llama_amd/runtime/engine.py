@@ -181,6 +181,7 @@ class DecodeEngine:
         self.cur_len = torch.zeros(1, **i32)
         self.sequences = torch.zeros(batch_size, max_length, **i32)
         self.key_mask: Optional[torch.Tensor] = None
+        self._key_mask_buf: Optional[torch.Tensor] = None
         self._graph = None
         self._graph_key = None
         self.keep_graph = False  # keep the captured graph's topology (runtime/benchmark.py counts its kernel nodes)
@@ -273,7 +274,11 @@ class DecodeEngine:
             held = 0
         else:
             self.kv_start.copy_(each(start))
-            self.key_mask = each(key_mask) if key_mask is not None else None
+            self.key_mask = None
+            if key_mask is not None:  # (a captured step reads the mask where the engine keeps it)
+                if self._key_mask_buf is None:
+                    self._key_mask_buf = torch.empty(self.b, self.max_length, dtype=torch.uint8, device=dev)
+                self.key_mask = self._key_mask_buf.copy_(each(key_mask))
             if n == 1:
                 logits = self._prefill_rows(ids, pos_dev, self.cache, self.kv_start, key_mask)
             else:

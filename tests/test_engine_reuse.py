@@ -67,3 +67,27 @@ def test_state_of_a_captured_step():
     greedy = state(do_sample=False)
     assert state(do_sample=False, seed=9, temperature=0.1, top_k=1, top_p=0.2) == greedy
     assert state(do_sample=False, eos_token_id=4) != greedy
+
+
+def holes(b, s, seed):
+    mask = (torch.rand(b, s, generator=torch.Generator().manual_seed(seed)) < 0.6).to(torch.int32)
+    mask[:, 0] = mask[:, -1] = 1
+    mask[:, s // 2] = 0
+    return mask
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("penalty", [1.0, 1.4])
+def test_masks_with_holes_of_the_present_call(device, penalty):
+    model, ids = model_of(device), prompts(4, 12)
+    kept = DecodeEngine(model, 4, 40)
+    gc = config(max_length=40, do_sample=False, repetition_penalty=penalty)
+    seen, places = set(), set()
+    for seed in (0, 1, 2, 1):
+        got = kept.run(ids, holes(4, 12, seed), gc).cpu().clone()
+        places.add(kept.key_mask.data_ptr())
+        torch.full((4, 40), 0, dtype=torch.uint8, device=device)  # (memory that an earlier call has given back is used again)
+        assert torch.equal(got, DecodeEngine(model, 4, 40).run(ids, holes(4, 12, seed), gc).cpu())
+        seen.add(tuple(got.reshape(-1).tolist()))
+        assert torch.equal(kept.run(ids, None, gc), DecodeEngine(model, 4, 40).run(ids, None, gc))
+    assert len(seen) == 3 and len(places) == 1  # (a captured step holds the mask's address)
