@@ -42,7 +42,8 @@ class LayerListLM:
         self.comm = NO_COMM
         self.vocab_local = config.vocab_size
         self.eps = config.norm_eps
-        self.blocks: List = []
+        self.weights_version = 0  # counts the loads: captured steps hold the weights' addresses
+        self.blocks = []
         self.embed: Optional[torch.Tensor] = None
         self.embed_scale = 1.0
         self.embed_norm: Optional[torch.Tensor] = None  # fp32 [D]: gain of an RMS norm on the embedding
@@ -54,6 +55,15 @@ class LayerListLM:
         self.head: Optional[torch.Tensor] = None
         if _do_init:
             self.load_state_dict(self.random_state_dict(config, seed))
+
+    @property
+    def blocks(self) -> List:
+        return self._blocks
+
+    @blocks.setter
+    def blocks(self, blocks: List) -> None:  # (every load makes them anew)
+        self._blocks = blocks
+        self.weights_version += 1
 
     # ------------------------------------------------------------------ family hooks
     @staticmethod

@@ -195,6 +195,7 @@ class LLaMAForCausalLM:
         self.layers: List[LayerWeights] = [LayerWeights() for _ in range(c.num_hidden_layers)]
         self.blocks = LLaMABlockCollection(self)  # reference FlaxLLaMABlockCollection (model.py:548)
         self._params_id = None
+        self.weights_version = 0  # counts the loads: captured steps hold the weights' addresses
         self.lm_head_f32: Optional[torch.Tensor] = None  # [V/tp, D] fp32 (precision='highest')
         if _do_init:
             self.init_random(seed=self.seed)
@@ -212,6 +213,7 @@ class LLaMAForCausalLM:
         """Load a reference-named parameter tree (Flax ``(in, out)`` kernel orientation, as
         returned by ``convert_llama_weights``). ``sharded=False``: the tree is the full
         model and this rank keeps its TP shard (partition rules of ``partition.py``)."""
+        self.weights_version += 1
         if not sharded:
             params = shard_tree(params, self.tp_rank, self.tp_size)
         dev = self.device
@@ -244,6 +246,7 @@ class LLaMAForCausalLM:
     def init_random(self, seed: int = 0, std: Optional[float] = None) -> "LLaMAForCausalLM":
         """Random-init every weight directly in the device layout (synthetic benchmarks).
         Norm weights are ones (folded), like Flax's RMSNorm init."""
+        self.weights_version += 1
         c = self.config
         std = c.initializer_range if std is None else std
         dev = self.device

@@ -338,7 +338,8 @@ class DecodeEngine:
     def _graph_state(self):
         # the graph records buffer addresses (the scratch workspaces, ops.workspace) and what a step takes as numbers from the settings
         gc = self.gc
-        return ((gc.seed, gc.temperature, gc.top_k, gc.top_p) if gc.do_sample else None, gc.pad_token_id, gc.eos_token_id, self.key_mask is not None, ops.workspace.generation, _fused_greedy(),
+        return ((gc.seed, gc.temperature, gc.top_k, gc.top_p) if gc.do_sample else None, gc.pad_token_id, gc.eos_token_id, self.model.weights_version,
+                self.key_mask is not None, ops.workspace.generation, _fused_greedy(),
                 ops.ARGMAX_FUSED_MIN_M, ops.SKINNY_ARGMAX, ops.QKV_ATTN, self.model.comm.reduce_dtype, self.rules.key(), self._prefix_state())
 
     def _prefix_state(self):

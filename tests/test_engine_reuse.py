@@ -9,10 +9,13 @@ DEVICES = ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)]
 V = 96
 
 
+def sizes():
+    return LLaMAConfig(vocab_size=V, hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+                       num_key_value_heads=1, max_sequence_length=128, rms_norm_eps=1e-5)
+
+
 def model_of(device):
-    cfg = LLaMAConfig(vocab_size=V, hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
-                      num_key_value_heads=1, max_sequence_length=128, rms_norm_eps=1e-5)
-    return LLaMAForCausalLM(cfg, device=device, _do_init=False).init_random(seed=3, std=0.12)
+    return LLaMAForCausalLM(sizes(), device=device, _do_init=False).init_random(seed=3, std=0.12)
 
 
 def prompts(b, s, seed=0):
@@ -91,3 +94,39 @@ def test_masks_with_holes_of_the_present_call(device, penalty):
         seen.add(tuple(got.reshape(-1).tolist()))
         assert torch.equal(kept.run(ids, None, gc), DecodeEngine(model, 4, 40).run(ids, None, gc))
     assert len(seen) == 3 and len(places) == 1  # (a captured step holds the mask's address)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_weights_of_the_present_call(device):
+    """``generate(params=...)`` and loading again: the engine kept for these sizes runs the weights that the model holds now."""
+    from helpers import build
+    cfg = sizes()
+    trees = [build(cfg, seed=s)[3] for s in (1, 2)]
+    ids = torch.randint(3, cfg.vocab_size, (2, 6), generator=torch.Generator().manual_seed(0), dtype=torch.int32)
+    gc = GenerationConfig(max_length=24, pad_token_id=0, eos_token_id=-1)
+    model = LLaMAForCausalLM(cfg, device=device, _do_init=False)
+    kept, seen, states = DecodeEngine(model, 2, 24), [], []
+    for i in (0, 1, 0):
+        model.load_params(trees[i])
+        got = kept.run(ids, None, gc).cpu().clone()
+        fresh = LLaMAForCausalLM(cfg, device=device, _do_init=False).load_params(trees[i])
+        assert torch.equal(got, DecodeEngine(fresh, 2, 24).run(ids, None, gc).cpu())
+        seen.append(tuple(got.reshape(-1).tolist()))
+        states.append(kept._graph_state())
+    assert len(set(seen)) == 2 and states[0] != states[1] != states[2]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_weights_of_layer_list_models(device):
+    import test_besulix
+    model, sd = test_besulix.build(test_besulix.cfg_full(), device)
+    other = {k: t.flip(0) if k == "embed" else t for k, t in sd.items()}
+    ids = torch.randint(3, 37, (2, 6), generator=torch.Generator().manual_seed(0), dtype=torch.int32)
+    gc = GenerationConfig(max_length=20, pad_token_id=0, eos_token_id=-1)
+    kept, seen = DecodeEngine(model, 2, 20), []
+    for weights in (sd, other, sd):
+        model.load_state_dict(weights)
+        got = kept.run(ids, None, gc).cpu().clone()
+        assert torch.equal(got, DecodeEngine(model, 2, 20).run(ids, None, gc).cpu())
+        seen.append((tuple(got.reshape(-1).tolist()), kept._graph_state()))
+    assert seen[0][0] == seen[2][0] != seen[1][0] and seen[0][1] != seen[1][1] != seen[2][1]
