@@ -49,16 +49,24 @@ class KVCache:
         return self.k.device
 
     def row_layout(self) -> cache_rows.RowLayout:
-        at = (self.k.data_ptr(), self.v.data_ptr())
+        starts = () if self.start is None else (self.start,)
+        at = tuple(t.data_ptr() for t in (self.k, self.v, *starts))
         if self._row_layout is None or self._row_layout[0] != at:
-            self._row_layout = at, cache_rows.RowLayout(self.batch_size, layers=(self.k, self.v))
+            self._row_layout = at, cache_rows.RowLayout(self.batch_size, layers=(self.k, self.v), state=starts)
         return self._row_layout[1]
 
     def copy_rows(self, src: Sequence[int], dst: Sequence[int], tokens: Optional[int] = None, to: Optional["KVCache"] = None) -> None:
         """Row ``dst[i]`` becomes row ``src[i]`` (-1: zeros) in every layer, its first ``tokens`` tokens (default: as many as the cache
         holds by its host counter): forks, reordering, moving live rows to the front. Every source is read as it was before the call; a row is
-        written once at most. ``to``: the rows written are those of another cache with the same layers (whose slot counter stays as it is).
-        One launch; up to some 300 rows also while a stream is captured, once the caches have copied rows before."""
+        written once at most. A padded row's ``start`` goes with it. ``to``: the rows written are those of another cache with the same layers
+        (whose slot counter stays as it is). One launch; up to some 300 rows also while a stream is captured, once the caches have copied
+        rows before."""
+        if isinstance(to, KVCache) and (self.start is None) != (to.start is None):
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first copy between a padded prefix and a cache without padding cannot be captured: make one before")
+            for cache in (self, to):
+                if cache.start is None:
+                    cache.start = torch.zeros(cache.batch_size, dtype=torch.int32, device=cache.device)
         _copy_rows(self, src, dst, tokens, to)
 
     def layer(self, i: int):
@@ -71,6 +79,7 @@ class KVCache:
     def reset(self) -> None:
         self.index = 0
         self.index_t.zero_()
+        self.start = None
 
     def clear(self) -> None:
         """``reset`` and zero the keys and values (after a failed step may have left non-finite rows)."""
@@ -120,6 +129,10 @@ class KVCacheRows:
     def index_t(self):
         return self.parent.index_t
 
+    @property
+    def start(self):
+        return None if self.parent.start is None else self.parent.start[self.b0:self.b1]
+
     def layer(self, i: int):
         return self.parent.k[i, self.b0:self.b1], self.parent.v[i, self.b0:self.b1]
 
@@ -131,20 +144,25 @@ class SharedPrefixCache:
     """A batch's own cache behind prefixes that its rows share: row ``b`` of ``B`` continues row ``b // (B / G)`` of ``prefix`` (a KVCache of
     ``G`` rows holding the prefixes' keys and values, read once for all of a prefix's rows: ``ops.prefix_attention``). Slots, ``index`` and
     ``layer(i)`` are those of ``own``; positions go on where the prefix ends. ``start`` / ``mask``: the prefixes' first keys (int32
-    ``[G]``) and the keys that count (uint8 ``[G, capacity]``). Anything that writes here writes to ``own`` alone."""
+    ``[G]``; left out: the prefix's own ``start``, as it is at each call) and the keys that count (uint8 ``[G, capacity]``). Anything that
+    writes here writes to ``own`` alone."""
 
     def __init__(self, prefix: KVCache, own, start: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
         if own.batch_size % prefix.batch_size:
             raise ValueError(f"{own.batch_size} rows are not a multiple of {prefix.batch_size} prefixes")
         if prefix.device != own.device:
             raise ValueError(f"the prefixes lie on {prefix.device}, the rows on {own.device}")
-        self.prefix, self.own, self.start, self.mask = prefix, own, start if start is not None else prefix.start, mask
+        self.prefix, self.own, self._start, self.mask = prefix, own, start, mask
         self.prefix_len = torch.full((prefix.batch_size,), prefix.index, dtype=torch.int32, device=prefix.device)
         self.batch_size, self.max_length = own.batch_size, own.max_length
 
     @property
     def device(self):
         return self.own.device
+
+    @property
+    def start(self) -> Optional[torch.Tensor]:
+        return self._start if self._start is not None else self.prefix.start
 
     @property
     def index(self):
@@ -188,7 +206,7 @@ class SharedPrefixCache:
             raise ValueError(f"rows {b0} .. {b1 - 1} hold some of one prefix's rows and others")
         part = SharedPrefixCache.__new__(SharedPrefixCache)
         part.prefix, part.own = self.prefix.rows(g0, g1), self.own.rows(b0, b1)
-        part.start, part.mask = (t[g0:g1] if t is not None else None for t in (self.start, self.mask))
+        part._start, part.mask = (t[g0:g1] if t is not None else None for t in (self._start, self.mask))
         part.prefix_len, part.batch_size, part.max_length = self.prefix_len[g0:g1], b1 - b0, self.max_length
         return part
 

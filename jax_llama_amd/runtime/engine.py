@@ -304,7 +304,6 @@ class DecodeEngine:
         if self.prefix.index + self.max_length > self.model.rope_length:
             raise ValueError(f"{self.prefix.index} + {self.max_length} tokens exceed the RoPE table ({self.model.rope_length})")
         self.cache.prefix_len.fill_(self.prefix.index)
-        self.cache.start = self.prefix.start
 
     def _prefill_rows(self, ids: torch.Tensor, pos_dev: torch.Tensor, cache, kv_start: torch.Tensor, key_mask: Optional[torch.Tensor]):
         """The prompt forward, in row chunks of at most PREFILL_TOKENS tokens: every kernel then sees at most the
