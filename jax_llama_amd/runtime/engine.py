@@ -44,7 +44,7 @@ class GenerationConfig:
     """Subset of HF ``GenerationConfig`` used by the reference (``generation.py:32-40``), and how the logits are changed before a token is
     chosen (``ops.process_logits``, in this order): ``repetition_penalty`` on the tokens of prompt and continuation,
     ``frequency_penalty`` / ``presence_penalty`` on those of the continuation, ``logit_bias`` (token -> number, or fp32 ``[V]``) and
-    ``suppress_tokens``, ``grammar``. ``num_return_sequences``: sampled continuations of each prompt, next to each other in the result."""
+    ``suppress_tokens``, ``grammar`` (settings that leave no token are refused). ``num_return_sequences``: sampled continuations of each prompt, next to each other in the result."""
 
     max_length: Optional[int] = None
     max_new_tokens: Optional[int] = None
@@ -193,7 +193,7 @@ class DecodeEngine:
         if self.rules.any:
             logits_local = self.rules.apply(logits_local, self.sequences, self.cur_len)
         nxt = _sample(self.model, logits_local, self.gc, self._gen, self.cur_len) if self.gc.do_sample else _greedy(self.model, logits_local)
-        self.rules.chosen(nxt)
+        self.rules.chosen(nxt, self.finished)
         return nxt
 
     def _update(self, nxt: torch.Tensor):

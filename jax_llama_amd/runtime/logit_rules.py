@@ -10,7 +10,9 @@ from .. import ops
 
 class TokenGrammar:
     """A finite automaton over token ids: ``next_state [states, V]`` (integers) holds the state after a token, -1 where a state forbids it. A
-    row starts in state ``start``; every state must allow a token (end tokens that may come are allowed like others)."""
+    row starts in state ``start``; every state must allow a token (end tokens that may come are allowed like others). Where suppressed
+    tokens leave a state that a row can come to without one, the generation is refused; a row whose logits leave it none (all -inf)
+    ends there, as behind an end token."""
 
     def __init__(self, next_state: torch.Tensor, start: int = 0):
         t = torch.as_tensor(next_state)
@@ -25,12 +27,33 @@ class TokenGrammar:
         self._on: Dict[torch.device, tuple] = {}
 
     def on(self, device) -> tuple:
-        """(next_state, allowed bits) on ``device``."""
+        """On ``device``: the states after each token, int32 ``[states + 1, V]`` with ``states`` (which stays itself) for forbidden ones, and
+        the allowed tokens' bits."""
         device = torch.device(device)
         if device not in self._on:
-            t = self.next_state.to(device)
-            self._on[device] = t, ops.pack_allowed(t >= 0)
+            n, v = self.next_state.shape
+            t = torch.empty(n + 1, v, dtype=torch.int32, device=device)
+            t[:n] = self.next_state
+            t[n] = n
+            allowed = ops.pack_allowed(t[:n] >= 0)
+            self._on[device] = t.masked_fill_(t < 0, n), allowed
         return self._on[device]
+
+    def check_open(self, closed: torch.Tensor, device) -> None:
+        """A ValueError if a row can come to a state that allows ``closed`` tokens (truth values ``[V]``) alone."""
+        table, n, opened = self.on(device)[0], self.next_state.shape[0], ~closed.to(device)
+        some = max(1, (1 << 26) // table.shape[1])  # states at a time
+        live = torch.cat([((table[a:min(n, a + some)] < n) & opened).any(1) for a in range(0, n, some)]).cpu()
+        seen = todo = set() if bool(live.all()) else {self.start}
+        while todo:
+            if not bool(live[sorted(todo)].all()):
+                raise ValueError(f"states {[s for s in sorted(todo) if not live[s]][:8]} of the grammar allow suppressed tokens alone")
+            at, todo = sorted(todo), set()
+            for a in range(0, len(at), some):
+                t = table[at[a:a + some]]
+                todo |= set(torch.unique(t[(t < n) & opened]).tolist())
+            todo -= seen
+            seen = seen | todo
 
 
 def as_bias(bias: Union[Dict[int, float], torch.Tensor, None], suppress: Optional[Sequence[int]], vocab: int) -> Optional[torch.Tensor]:
@@ -66,7 +89,7 @@ class LogitRules:
         self._mask_buf: Optional[torch.Tensor] = None
         self._bias_buf: Optional[torch.Tensor] = None
         self.max_length = max_length
-        self.bias = self.grammar = self.config = None
+        self.bias = self.grammar = self.table = self.allowed = None
         self.prompt_len = 0
 
     @property
@@ -79,6 +102,9 @@ class LogitRules:
         vocab = v * self.model.comm.size
         bias = as_bias(gc.logit_bias, gc.suppress_tokens, vocab)
         self.bias = None
+        closed = None if bias is None else bias == float("-inf")
+        if closed is not None and bool(closed.all()):
+            raise ValueError("every token is suppressed")
         if bias is not None:
             if self._bias_buf is None:
                 self._bias_buf = torch.empty(v, dtype=torch.float32, device=dev)
@@ -87,7 +113,9 @@ class LogitRules:
         if self.grammar is not None:
             if self.grammar.next_state.shape[1] != vocab:
                 raise ValueError(f"the grammar is over {self.grammar.next_state.shape[1]} tokens, the model over {vocab}")
-            self.grammar.on(dev)
+            if closed is not None and bool(closed.any()):
+                self.grammar.check_open(closed, dev)
+            self.table, self.allowed = self.grammar.on(dev)
             self.state.fill_(self.grammar.start)
         self.penalties = dict(repetition_penalty=float(gc.repetition_penalty), presence_penalty=float(gc.presence_penalty),
                               frequency_penalty=float(gc.frequency_penalty))
@@ -115,13 +143,15 @@ class LogitRules:
         kw = dict(self.penalties, history=sequences, length=cur_len, start=self.start, history_mask=self.mask,
                   prompt_len=self.prompt_len) if self.penalised else {}
         if self.grammar is not None:
-            kw.update(allowed=self.grammar.on(logits.device)[1], allowed_rows=self.state)
+            kw.update(allowed=self.allowed, allowed_rows=self.state)
         return ops.process_logits(logits, vocab_start=self.vocab0, bias=self.bias, out=logits, **kw)
 
-    def chosen(self, tokens: torch.Tensor) -> None:
-        """The rows' next tokens move their grammar states on (a finished row's are not looked at any more)."""
+    def chosen(self, tokens: torch.Tensor, finished: torch.Tensor) -> None:
+        """The rows' next tokens move their grammar states on (a finished row's are not looked at any more). A token that the grammar
+        forbids is the choice among -inf alone: the row is ``finished`` before it is said."""
         if self.grammar is None:
             return
-        table = self.grammar.on(tokens.device)[0]
-        at = self.state.clamp(min=0).long() * table.shape[1] + tokens.long()
-        self.state.copy_(table.reshape(-1).index_select(0, at))
+        states, vocab = self.table.shape
+        at = self.state.long().mul_(vocab).add_(tokens.clamp(0, vocab - 1))
+        torch.index_select(self.table.reshape(-1), 0, at, out=self.state)
+        finished.bitwise_or_(self.state == states - 1)
