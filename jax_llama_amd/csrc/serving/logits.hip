@@ -32,18 +32,19 @@ struct Penalties {
   }
 };
 
-// fn(column within the chunk, place) for the places of the row's history in this chunk, eight of them under way per thread
+// fn(column within the chunk, place) for the places of the row's history in this chunk, eight of them under way per thread. Places are
+// unsigned: `to` is below 2^31, so that a thread's next place past it does not wrap.
 template <class F>
 JLA_DEV void for_history(const LogitsArgs& a, int row, int c0, int n, F fn) {
-  const int to = min(a.length ? a.length[0] : a.length0, a.L);
+  const unsigned to = (unsigned)max(min(a.length ? a.length[0] : a.length0, a.L), 0);
   const int32_t* h = a.history + row * a.ldh;
   const uint8_t* m = a.hmask ? a.hmask + row * a.ldm : nullptr;
   const unsigned lowest = (unsigned)a.vocab0 + (unsigned)c0;
-  for (int i = max(a.start ? a.start[row] : 0, 0) + 4 * (int)threadIdx.x; i < to; i += 8 * LG_THREADS) {
+  for (unsigned i = min((unsigned)max(a.start ? a.start[row] : 0, 0), to) + 4 * threadIdx.x; i < to; i += 8 * LG_THREADS) {
     unsigned t[2][4];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int at = i + 4 * LG_THREADS * g;
+      const unsigned at = i + 4 * LG_THREADS * g;
       if (at + 4 <= to) {
         const i32x4u v = *reinterpret_cast<const i32x4u*>(h + at);
 #pragma unroll
@@ -57,8 +58,8 @@ JLA_DEV void for_history(const LogitsArgs& a, int row, int c0, int n, F fn) {
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int at = i + 4 * LG_THREADS * g + e;
-        if (t[g][e] < (unsigned)n && (!m || m[at])) fn(t[g][e], at);
+        const unsigned at = i + 4 * LG_THREADS * g + e;
+        if (t[g][e] < (unsigned)n && (!m || m[at])) fn(t[g][e], (int)at);
       }
   }
 }

@@ -164,7 +164,7 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
       * tokens that are not ``allowed`` become -inf, whatever stood there.
 
     ``history`` int32 ``[B, L]`` holds the tokens; row ``b``'s are the places ``start[b] <= i < length`` (``start`` int32 ``[B]``, else 0;
-    ``length`` an int or a device int32[1], so that a captured step sees the present one) with ``history_mask[b, i] != 0`` (uint8). Ids
+    any numbers: a row that starts behind the end has no history; ``length`` an int or a device int32[1], so that a captured step sees the present one) with ``history_mask[b, i] != 0`` (uint8). Ids
     outside the columns are passed over. A penalty is a number or fp32 ``[B]``. ``allowed``: int32 bits ``[masks, words]``
     (``pack_allowed``), one mask for all, one per row, or row ``allowed_rows[b]`` of them (int32 ``[B]``; an index outside the masks allows
     everything). ``vocab_start``: token id of column 0 (a vocabulary shard); ``bias`` has the shard's columns, ``allowed`` all ids.
