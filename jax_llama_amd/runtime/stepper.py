@@ -52,8 +52,12 @@ class SequenceStepper:
             raise ValueError(f"request {new!r} is live already")
         held = self._live[rid]
         cache = self._row(new)
-        held.copy_rows([0], [0], to=cache)
-        cache.advance(held.index)
+        try:
+            held.copy_rows([0], [0], to=cache)
+            cache.advance(held.index)
+        except BaseException:
+            self.end(new)  # (an empty request by that name would go on without its context)
+            raise
 
     # ---------------------------------------------------------------- steps
     def feed(self, rid: str, tokens: Sequence[int], want: Sequence[int] = ()) -> Optional[torch.Tensor]:
