@@ -348,8 +348,8 @@ class DecodeEngine:
         return (c.prefix.k.data_ptr(), c.prefix.v.data_ptr(), *(t.data_ptr() if t is not None else 0 for t in (c.start, c.mask)))
 
     def nbytes(self) -> int:
-        """Of the caches it keeps alive (a prefix counts in each engine behind it)."""
-        return sum(c.nbytes() for c in (self.cache, self.prompt_cache, self.prefix) if c is not None)
+        """Of the caches it keeps alive."""
+        return _held_bytes([self])
 
     def _ensure_graph(self):
         if self._graph is not None and self._graph_key == self._graph_state():
@@ -446,6 +446,14 @@ def _engine_budget(model) -> int:
     return 8 << 30
 
 
+def _held_bytes(engines, prefix: Optional[KVCache] = None) -> int:
+    """Of the caches that ``engines`` (and ``prefix``) keep alive: a prefix counts once, however many engines are behind it."""
+    engines = list(engines)
+    prefixes = {id(p): p for p in (prefix, *(e.prefix for e in engines)) if p is not None}
+    own = [c for e in engines for c in (e.cache, e.prompt_cache) if c is not None]
+    return sum(c.nbytes() for c in (*own, *prefixes.values()))
+
+
 def get_engine(model, batch_size: int, max_length: int, samples: int = 1, prompt_len: int = 0, prefix: Optional[KVCache] = None) -> DecodeEngine:
     """Per-(model, B, max_length) engines (each owns a KV cache and a captured decode graph; of several samples per prompt, and behind a
     prefix, engines of their own), kept in LRU order and bounded by the bytes of their KV caches."""
@@ -461,14 +469,9 @@ def get_engine(model, batch_size: int, max_length: int, samples: int = 1, prompt
     else:
         tokens = batch_size * prompt_len + rows * (max_length - prompt_len) if shared else rows * max_length
         need = model.config.num_hidden_layers * 2 * tokens * model.n_kv_heads * model.head_dim * 2
-    if prefix is not None:
-        need += prefix.nbytes()
     budget = _engine_budget(model)
-    held = sum(e.nbytes() for e in _ENGINES.values())
-    while _ENGINES and held + need > budget:
-        _, old = _ENGINES.popitem(last=False)
-        held -= old.nbytes()
-        del old
+    while _ENGINES and _held_bytes(_ENGINES.values(), prefix) + need > budget:
+        _ENGINES.popitem(last=False)
     eng = DecodeEngine(model, batch_size, max_length, samples=samples, prompt_len=prompt_len, prefix=prefix)
     _ENGINES[key] = eng
     return eng

@@ -130,3 +130,32 @@ def test_weights_of_layer_list_models(device):
         assert torch.equal(got, DecodeEngine(model, 2, 20).run(ids, None, gc).cpu())
         seen.append((tuple(got.reshape(-1).tolist()), kept._graph_state()))
     assert seen[0][0] == seen[2][0] != seen[1][0] and seen[0][1] != seen[1][1] != seen[2][1]
+
+
+def test_bytes_of_engines_behind_one_prefix(monkeypatch):
+    """A prefix counts once, however many engines keep it alive, and as long as one of them does."""
+    from jax_llama_amd.runtime import engine
+    model = model_of("cpu")
+    big, other = model.encode_prefix(prompts(1, 60)), model.encode_prefix(prompts(1, 60, seed=1))
+
+    def call(prefix, b):
+        model.generate(prompts(b, 4), None, config(max_length=8), prefix=prefix)
+
+    def kept():
+        return [(e.prefix, e.b) for e in engine._ENGINES.values()]
+
+    engine._ENGINES.clear()
+    own = model.init_cache(1, 8).nbytes()
+    monkeypatch.setattr(engine, "_engine_budget", lambda m: big.nbytes() + 6 * own)
+    for b in (1, 2, 3):  # 6 rows of own keys and one prefix
+        call(big, b)
+    engines = list(engine._ENGINES.values())
+    assert kept() == [(big, 1), (big, 2), (big, 3)] and engine._held_bytes(engines) == big.nbytes() + 6 * own
+    for b in (1, 2, 3):  # the same engines again
+        call(big, b)
+    assert list(engine._ENGINES.values()) == engines
+    call(big, 4)  # 3 + 4 rows are too many, the prefix stays
+    assert kept() == [(big, 4)]
+    call(other, 1)  # another prefix does not fit beside it
+    assert kept() == [(other, 1)] and engine._held_bytes(engine._ENGINES.values()) == big.nbytes() + own
+    engine._ENGINES.clear()
