@@ -140,10 +140,15 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
     word ``v // 32``; bits past ``V`` are 0."""
     _need(allowed.dim() == 2, "pack_allowed takes [masks, V]")
     n, v = allowed.shape
-    bits = torch.zeros(n, -(-v // 32) * 32, dtype=torch.int64, device=allowed.device)
-    bits[:, :v] = allowed != 0
-    words = (bits.view(n, -1, 32) << torch.arange(32, device=allowed.device)).sum(-1)
-    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    words = torch.empty(n, -(-v // 32), dtype=torch.int32, device=allowed.device)
+    place = torch.arange(32, device=allowed.device)
+    some = max(1, (1 << 22) // max(v, 1))  # masks at a time: 64 bits a token on the way
+    for a in range(0, n, some):
+        bits = torch.zeros(min(some, n - a), words.shape[1] * 32, dtype=torch.int64, device=allowed.device)
+        bits[:, :v] = allowed[a:a + some] != 0
+        packed = (bits.view(len(bits), -1, 32) << place).sum(-1)
+        words[a:a + some] = torch.where(packed >= 1 << 31, packed - (1 << 32), packed)
+    return words
 
 
 def _neutral(v: Number, one: float) -> bool:

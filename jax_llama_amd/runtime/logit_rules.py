@@ -12,7 +12,8 @@ class TokenGrammar:
     """A finite automaton over token ids: ``next_state [states, V]`` (integers) holds the state after a token, -1 where a state forbids it. A
     row starts in state ``start``; every state must allow a token (end tokens that may come are allowed like others). Where suppressed
     tokens leave a state that a row can come to without one, the generation is refused; a row whose logits leave it none (all -inf)
-    ends there, as behind an end token."""
+    ends there, as behind an end token. A device that it is used on keeps its tables: 4 (states + 1) V bytes of states and states V / 8 of
+    masks (2000 states over 128256 tokens: 1.06 GB)."""
 
     def __init__(self, next_state: torch.Tensor, start: int = 0):
         t = torch.as_tensor(next_state)

@@ -81,3 +81,46 @@ def test_states_of_a_grammar_with_its_end():
     nxt, allowed = g.on("cpu")
     assert nxt.shape == (3, V) and allowed.shape == (2, V // 32)
     assert nxt[0, 3] == 1 and nxt[1, 4] == 0 and int((nxt != 2).sum()) == 2 and bool((g.next_state >= -1).all())
+
+
+class _Largest(torch.utils._python_dispatch.TorchDispatchMode):
+    """The largest tensor that the operations within give back, in bytes."""
+
+    def __init__(self):
+        super().__init__()
+        self.bytes = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        for t in out if isinstance(out, (tuple, list)) else (out,):
+            if torch.is_tensor(t):
+                self.bytes = max(self.bytes, t.untyped_storage().nbytes())
+        return out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,v", [(1, 1), (3, 32), (5, 33), (7, 100), (1200, 32001), (2, 2 ** 21 + 5)])
+def test_packed_masks(device, n, v):
+    """Against the definition; what it takes on the way stays within 64 MiB or a few times the truth values."""
+    from jax_llama_amd import ops
+    mask = (torch.rand(n, v, generator=torch.Generator().manual_seed(1)) < 0.3).to(device)
+    with _Largest() as most:
+        words = ops.pack_allowed(mask)
+    assert words.dtype == torch.int32 and words.shape == (n, -(-v // 32))
+    assert most.bytes <= max(2 ** 26, 16 * (v + 31))
+    at = torch.arange(v, device=device)
+    for a in range(0, n, 200):
+        assert torch.equal((words[a:a + 200][:, at // 32] >> (at % 32).to(torch.int32)) & 1 == 1, mask[a:a + 200])
+    if v % 32:
+        assert not bool((words[:, -1] >> (v % 32) & ((1 << (32 - v % 32)) - 1)).any())  # (bits past V)
+
+
+def test_packed_masks_of_other_types():
+    from jax_llama_amd import ops
+    mask = torch.tensor([[0, 2, 0, -1], [1, 0, 0, 0]])
+    for t in (mask, mask.float(), mask.to(torch.uint8), mask.t().contiguous().t()):
+        assert ops.pack_allowed(t).tolist() == [[10], [1]]
+    assert ops.pack_allowed(torch.zeros(0, 40)).shape == (0, 2)
+    assert ops.pack_allowed(torch.ones(1, 32)).tolist() == [[-1]]
+    with pytest.raises(ValueError):
+        ops.pack_allowed(torch.zeros(4))
