@@ -359,7 +359,8 @@ class LLaMAForCausalLM:
 
     def share_prefix(self, prefix: KVCache, batch_size: int, max_length: int) -> SharedPrefixCache:
         """A cache of ``batch_size`` rows (``past_key_values``) of ``max_length`` own tokens each behind the prefixes in ``prefix``; row ``b``
-        continues prefix ``b // (batch_size / G)``. Positions go on at the prefix's number of real tokens."""
+        continues prefix ``b // (batch_size / G)``. Positions go on at the prefix's number of real tokens; ``attention_mask`` is of the rows'
+        own slots: the call's, all up to them, or all ``max_length``."""
         if prefix.index + max_length > self.rope_length:
             raise ValueError(f"{prefix.index} + {max_length} tokens exceed the RoPE table ({self.rope_length})")
         return SharedPrefixCache(prefix, self.init_cache(batch_size, max_length))
@@ -456,6 +457,8 @@ class LLaMAForCausalLM:
             return ids, pos, cache, slot0, torch.zeros(b, dtype=torch.int32, device=self.device), None
         else:
             mask = _t(attention_mask).to("cpu").to(torch.int32)
+            if isinstance(cache, SharedPrefixCache) and mask.shape[1] not in (s, t_valid, cache.max_length):
+                raise ValueError(f"attention_mask of shape {tuple(mask.shape)} behind a shared prefix: of the rows' own slots ({s}, {t_valid} or {cache.max_length})")
             if mask.shape[1] >= t_valid:
                 mask = mask[:, :t_valid]
             elif mask.shape[1] == s:

@@ -134,3 +134,30 @@ def test_captured_copies_of_a_padded_prefix():
         torch.cuda.synchronize()
         assert fresh.start.tolist() == want
     assert torch.equal(fresh.k, prefix.k)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_masks_of_the_rows_behind_a_prefix(device):
+    """``attention_mask`` is of the rows' own slots: the portion's, all so far, or the cache's. One over the prefix too is refused (its
+    first columns would be taken for the rows' own)."""
+    model, head, ids = model_of(device), prompts(1, 20), prompts(2, 6, seed=2)
+    prefix, pad = model.encode_prefix(head), padded(2, 0, s=6)
+    pos = torch.cat([torch.arange(18, 24)[None], torch.arange(20, 26)[None]]).to(torch.int32)
+
+    def call(mask, room=30):
+        return model(ids, attention_mask=mask, past_key_values=model.share_prefix(prefix, 2, room), position_ids=pos).logits
+
+    want = call(pad)
+    whole = torch.cat([pad, torch.ones(2, 24, dtype=torch.int32)], 1)
+    assert torch.equal(call(whole)[:, 2:], want[:, 2:])
+    assert not torch.equal(call(None), want)
+    for mask in (torch.cat([torch.ones(2, 20, dtype=torch.int32), pad], 1), torch.cat([torch.ones(2, 20, dtype=torch.int32), whole], 1), pad[:, 1:]):
+        with pytest.raises(ValueError):
+            call(mask)
+    # a second portion: its own columns, or all the rows' slots so far
+    outs = []
+    for mask in (torch.ones(2, 3, dtype=torch.int32), torch.cat([pad, torch.ones(2, 3, dtype=torch.int32)], 1)):
+        shared = model.share_prefix(prefix, 2, 30)
+        model(ids, attention_mask=pad, past_key_values=shared, position_ids=pos)
+        outs.append(model(ids[:, :3], attention_mask=mask, past_key_values=shared, position_ids=pos[:, -1:] + torch.arange(1, 4)).logits)
+    assert not torch.equal(*outs)  # (the first takes the padding of the portion before for keys)
