@@ -78,7 +78,7 @@ struct RowSpan {             // a tensor, or several equal ones (layers) at one 
 // Steps (a, b) of a chain run in order, each thread at its own place of every row: b >= 0: row a (ROW_ZERO: zeros, ROW_SAVED: the saved
 // one) goes to row b; b == ROW_SAVED: row a is saved. No chain writes a row that another one reads or writes.
 constexpr int ROW_ZERO = -1, ROW_SAVED = -2;
-constexpr int ROW_STEPS = 320, ROW_FEW = 32, ROW_SPANS = 2;  // what travels as the kernel's argument
+constexpr int ROW_STEPS = 320, ROW_FEW = 32, ROW_SPANS = 3;  // what travels as the kernel's argument (keys, values, rows' starts)
 template <int STEPS>
 struct RowProgramOf {
   int32_t step[2 * STEPS];

@@ -41,15 +41,29 @@ class KVCache:
         self.max_length = max_length
         self.index = 0  # host mirror of the number of filled slots
         self.index_t = torch.zeros(1, dtype=torch.int32, device=device)
-        self.start: Optional[torch.Tensor] = None  # int32 [B]: a left-padded prefix's first real slot of each row (``encode_prefix``)
+        self._start: Optional[torch.Tensor] = None  # keeps its place once there (captured copies write it); zeros where nothing is padded
+        self._padded = False
         self._row_layout = None
 
     @property
     def device(self):
         return self.k.device
 
+    @property
+    def start(self) -> Optional[torch.Tensor]:
+        """int32 ``[B]``: a left-padded prefix's first real slot of each row (``encode_prefix``); None: every row begins at slot 0."""
+        return self._start if self._padded else None
+
+    @start.setter
+    def start(self, start: Optional[torch.Tensor]) -> None:
+        self._padded = start is not None
+        if self._start is None and start is not None:
+            self._start = torch.zeros(self.batch_size, dtype=torch.int32, device=self.device)
+        if self._start is not None:
+            self._start.zero_() if start is None else self._start.copy_(start)
+
     def row_layout(self) -> cache_rows.RowLayout:
-        starts = () if self.start is None else (self.start,)
+        starts = () if self._start is None else (self._start,)
         at = tuple(t.data_ptr() for t in (self.k, self.v, *starts))
         if self._row_layout is None or self._row_layout[0] != at:
             self._row_layout = at, cache_rows.RowLayout(self.batch_size, layers=(self.k, self.v), state=starts)
@@ -61,13 +75,15 @@ class KVCache:
         written once at most. A padded row's ``start`` goes with it. ``to``: the rows written are those of another cache with the same layers
         (whose slot counter stays as it is). One launch; up to some 300 rows also while a stream is captured, once the caches have copied
         rows before."""
-        if isinstance(to, KVCache) and (self.start is None) != (to.start is None):
-            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the first copy between a padded prefix and a cache without padding cannot be captured: make one before")
-            for cache in (self, to):
-                if cache.start is None:
-                    cache.start = torch.zeros(cache.batch_size, dtype=torch.int32, device=cache.device)
+        if isinstance(to, KVCache):
+            for cache, other in ((self, to), (to, self)):
+                if cache._start is None and other._start is not None:
+                    if cache.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("the first copy between a padded prefix and a cache without padding cannot be captured: make one before")
+                    cache._start = torch.zeros(cache.batch_size, dtype=torch.int32, device=cache.device)
         _copy_rows(self, src, dst, tokens, to)
+        if isinstance(to, KVCache):
+            to._padded = to._padded or self._padded
 
     def layer(self, i: int):
         return self.k[i], self.v[i]

@@ -161,3 +161,29 @@ def test_masks_of_the_rows_behind_a_prefix(device):
         model(ids, attention_mask=pad, past_key_values=shared, position_ids=pos)
         outs.append(model(ids[:, :3], attention_mask=mask, past_key_values=shared, position_ids=pos[:, -1:] + torch.arange(1, 4)).logits)
     assert not torch.equal(*outs)  # (the first takes the padding of the portion before for keys)
+
+
+@pytest.mark.gpu
+def test_captured_copies_outlive_what_the_caches_were():
+    """The starts keep their place: a replay after the caches were emptied, filled anew and copied without padding writes rows of these."""
+    model = model_of("cuda:0")
+    prefix, target = model.encode_prefix(prompts(2, 13), padded(6, 0, s=13)), model.init_cache(2, 13)
+    prefix.copy_rows([0, 1], [0, 1], to=target)
+    at = [t.data_ptr() for t in (prefix.start, target.start)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        prefix.copy_rows([1, 0], [0, 1], to=target)
+    for pads in ((3, 1), (0, 5)):
+        prefix.reset()
+        target.reset()
+        assert prefix.start is None and target.start is None
+        prefix.copy_rows([0], [0], to=target, tokens=13)  # (nothing is padded)
+        assert target.start is None
+        other = model.encode_prefix(prompts(2, 13, seed=sum(pads)), padded(*pads, s=13))
+        other.copy_rows([0, 1], [0, 1], to=prefix)
+        assert prefix.start.tolist() == list(pads)
+        graph.replay()
+        prefix.copy_rows([0], [0], to=target, tokens=0)  # (the host learns of the padding)
+        torch.cuda.synchronize()
+        assert target.start.tolist() == [pads[0], pads[0]] and torch.equal(target.k[:, 1], prefix.k[:, 0]) and torch.equal(target.k[:, 0], prefix.k[:, 1])
+        assert [t.data_ptr() for t in (prefix.start, target.start)] == at
