@@ -71,7 +71,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
         ``[G, P]`` on the device; left out: all ``P`` keys);
       * its row's own keys ``kv_start[b] <= j <= slot0 + s`` (``slot0``: an int or a device int32[1], ``kv_start`` int32 ``[B]``).
 
-    A query with no key gives zeros. What lies at places that no query of the call attends may be anything, NaN included; a value
+    A query with no key gives zeros. Maxima and sums are in 32 bits; on the GPU each weight is rounded to bf16 for the product with
+    the values. What lies at places that no query of the call attends may be anything, NaN included; a value
     that some query attends has to be finite for the queries of its row before it. Keys and values may be views whose heads and rows
     are strided (the tokens of a head follow one another). ``out_packed``: see ``attention``, up to 64 rows."""
     if q.device.type == "cuda":
@@ -169,7 +170,8 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
       * tokens that are not ``allowed`` become -inf, whatever stood there.
 
     ``history`` int32 ``[B, L]`` holds the tokens; row ``b``'s are the places ``start[b] <= i < length`` (``start`` int32 ``[B]``, else 0;
-    any numbers: a row that starts behind the end has no history; ``length`` an int or a device int32[1], so that a captured step sees the present one) with ``history_mask[b, i] != 0`` (uint8). Ids
+    any numbers: a row that starts behind the end has no history; ``length`` an int or a device int32[1], so that a captured step sees the
+    present one) with ``history_mask[b, i] != 0`` (uint8). Ids
     outside the columns are passed over. A penalty is a number or fp32 ``[B]``. ``allowed``: int32 bits ``[masks, words]``
     (``pack_allowed``), one mask for all, one per row, or row ``allowed_rows[b]`` of them (int32 ``[B]``; an index outside the masks allows
     everything). ``vocab_start``: token id of column 0 (a vocabulary shard); ``bias`` has the shard's columns, ``allowed`` all ids.
